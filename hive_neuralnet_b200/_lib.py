@@ -14,11 +14,11 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
 LIB_PATH = os.path.join(PKG_DIR, "libhive_b200.so")
 CSRC = os.path.join(PKG_DIR, "csrc")
-SOURCES = ["hv_kernels.cu"]
+SOURCES = ["hv_kernels.cu", "hv_train.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
+    "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "--threads", "0",
 ]
 
 HV_OK = 0
@@ -57,8 +57,20 @@ class HvTree(C.Structure):
         ("max_nodes", C.c_int32)]
 
 
+class HvAttention(C.Structure):
+    """hv_attention of include/hive_b200.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _i64 * 3), ("k_stride", _i64 * 3),
+                ("v_stride", _i64 * 3), ("token_q", _vp), ("token_r", _vp), ("token_z", _vp), ("token_mask", _vp),
+                ("token_stride", _i64 * 4), ("dq_bias", _vp), ("dr_bias", _vp), ("dz_bias", _vp), ("batch", _i64),
+                ("tokens", C.c_int32), ("queries", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32),
+                ("coord_clip", C.c_int32), ("height_clip", C.c_int32), ("dtype", C.c_int32),
+                ("table_dtype", C.c_int32), ("scale", C.c_float)]
+
+
 _tp = C.POINTER(HvTree)
+_ap = C.POINTER(HvAttention)
 _f = C.c_float
+_sz = C.c_size_t
 
 _SIGNATURES = {
     "hv_mcts_select": ([_tp, _int, _vp, _vp, _vp, _vp, _vp, _int, _int, _f, _int, _int, _int, _f, _f,
@@ -114,6 +126,16 @@ _SIGNATURES = {
     "hv_check_results": ([_vp, _i64, _vp, _vp], _int),
     "hv_compute_centroids": ([_vp, _i64, _vp, _vp], _int),
     "hv_legal_moves_to_actions": ([_vp, _vp, _vp, _i64, _vp, _vp], _int),
+    "hv_layer_norm_forward": ([_vp, _vp, _vp, _vp, _i64, _int, _int, _int, _f, _vp, _vp, _vp, _vp, _vp], _int),
+    "hv_layer_norm_workspace_bytes": ([_i64, _int, _int, _vp], _int),
+    "hv_layer_norm_backward": ([_vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _int, _int, _vp, _vp, _vp, _vp, _sz, _vp],
+                               _int),
+    "hv_adamw_step": ([_vp, _vp, _vp, _int, _int, _vp, _vp, _vp, _vp, _int, _f, _f, _f, _f, _f, _f, _f, _f,
+                       C.c_uint32, _vp], _int),
+    "hv_adamw_state_values": ([_vp, _vp, _i64, _int, _vp, _vp], _int),
+    "hv_relative_attention_sizes": ([_ap, _vp, _vp, _vp], _int),
+    "hv_relative_attention_forward": ([_ap, _vp, _vp, _vp, _sz, _vp], _int),
+    "hv_relative_attention_backward": ([_ap, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp], _int),
     "hv_generate_positions": ([C.c_uint64, _i64, _i64, _int, _int, _vp, _vp], _int),
 }
 

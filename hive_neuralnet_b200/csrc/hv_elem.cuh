@@ -1,0 +1,61 @@
+// hv_elem.cuh -- element types of the training operators: conversions between
+// the stored type (fp32, fp16, bf16) and the fp32 arithmetic, vector loads.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace hv {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// N consecutive elements moved as one memory word (N * sizeof(T) bytes, a
+// power of two up to 16, naturally aligned).
+template <typename T, int N>
+struct alignas(N * sizeof(T)) Vec {
+    T x[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* p, float* out) {
+    const Vec<T, N> v = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+    for (int i = 0; i < N; i++) out[i] = to_f32(v.x[i]);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const float* in) {
+    Vec<T, N> v;
+#pragma unroll
+    for (int i = 0; i < N; i++) v.x[i] = from_f32<T>(in[i]);
+    *reinterpret_cast<Vec<T, N>*>(p) = v;
+}
+
+// A value of a small fp32-or-T parameter tensor (weights, bias tables).
+template <typename T>
+__device__ __forceinline__ float load_param(const void* p, int64_t i, bool is_f32) {
+    return is_f32 ? static_cast<const float*>(p)[i] : to_f32(static_cast<const T*>(p)[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_param(void* p, int64_t i, bool is_f32, float x) {
+    if (is_f32)
+        static_cast<float*>(p)[i] = x;
+    else
+        static_cast<T*>(p)[i] = from_f32<T>(x);
+}
+
+}  // namespace hv

@@ -1,0 +1,355 @@
+// hv_train.cu -- the training operators' kernels and their C-ABI entry points
+// (declared in include/hive_b200.h): relative attention, layer norm, AdamW.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <initializer_list>
+#include <mutex>
+#include <type_traits>
+
+#include "hv_adamw.cuh"
+#include "hv_attn.cuh"
+#include "hv_norm.cuh"
+#include "../../include/hive_b200.h"
+
+namespace hv {
+
+static inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+static inline int launched() { return cudaGetLastError() == cudaSuccess ? HV_OK : HV_ECUDA; }
+
+static inline size_t elem_bytes(int dtype) { return dtype == HV_F32 ? 4 : 2; }
+
+static int sm_count() {
+    static int n[64];
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n[dev] = 0;
+    return n[dev];
+}
+
+// Calls f with a value of the element type.
+template <typename F>
+static int by_type(int dtype, F f) {
+    switch (dtype) {
+        case HV_F32: return f(float());
+        case HV_F16: return f(__half());
+        case HV_BF16: return f(__nv_bfloat16());
+        default: return HV_EINVAL;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+constexpr int kNormMaxWidth = kNormMaxThreads * kNormValues;
+constexpr int kNormBlocksPerSm = 4;
+
+struct NormShape {
+    int V, K, G, threads;
+};
+
+// V values a vector where rows and pointers allow 16-byte vectors, else 1.  A
+// row goes to the fewest threads of a warp that hold it at up to 16 values
+// each, or to a block where a warp cannot hold it.
+static bool norm_shape(int C, int dtype, bool vec, NormShape* s) {
+    s->V = vec ? (int)(16 / elem_bytes(dtype)) : 1;
+    const int n = (C + s->V - 1) / s->V;  // vectors of a row
+    s->G = 1;
+    while (s->G < 32 && s->G < n) s->G *= 2;
+    s->threads = kNormThreads;
+    if (n * s->V > 32 * kNormValues) {
+        s->threads = 128;
+        while (s->threads < kNormMaxThreads && n * s->V > s->threads * (kNormValues / 2)) s->threads *= 2;
+        s->G = s->threads;
+    }
+    s->K = 1;
+    while (s->K * s->G < n) s->K *= 2;
+    return s->K * s->V <= kNormValues;
+}
+
+static bool norm_vec(int C, int dtype, std::initializer_list<const void*> ptrs) {
+    bool ok = C * elem_bytes(dtype) % 16 == 0;
+    for (const void* p : ptrs) ok = ok && aligned(p, 16);
+    return ok;
+}
+
+template <typename T, bool BACK>
+static int launch_norm(const NormArgs& a, const NormShape& s, int grid, cudaStream_t st) {
+    auto go = [&](auto kernel) {
+        kernel<<<grid, s.threads, 0, st>>>(a);
+        return launched();
+    };
+    constexpr int V = 16 / sizeof(T);
+#define HV_NORM(VV, KK)                                        \
+    if constexpr (VV * KK <= kNormValues)                      \
+        if (s.V == VV && s.K == KK) {                          \
+            if constexpr (BACK) return go(k_norm_backward<T, VV, KK>); \
+            else return go(k_norm_forward<T, VV, KK>);         \
+        }
+    HV_NORM(V, 1)
+    HV_NORM(V, 2)
+    HV_NORM(V, 4)
+    HV_NORM(1, 1)
+    HV_NORM(1, 2)
+    HV_NORM(1, 4)
+    HV_NORM(1, 8)
+    HV_NORM(1, 16)
+#undef HV_NORM
+    return HV_EINVAL;
+}
+
+static int norm_grid(const NormShape& s, int64_t rows) {
+    const int64_t blocks = (rows + s.threads / s.G - 1) / (s.threads / s.G), cap = (int64_t)sm_count() * kNormBlocksPerSm;
+    return (int)(blocks < cap ? blocks : cap);
+}
+
+// ---------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------
+static size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+static bool attn_ok(const hv_attention* a) {
+    if (!a || a->batch < 0 || a->tokens < 0 || a->queries < 0 || a->queries > a->tokens || a->heads < 1) return false;
+    if (a->head_dim < 1 || a->head_dim > HV_ATTN_MAX_HEAD_DIM || a->dtype < 0 || a->dtype > 2) return false;
+    if (a->table_dtype != HV_F32 && a->table_dtype != a->dtype) return false;
+    if (a->coord_clip < 0 || a->coord_clip > HV_ATTN_MAX_CLIP || a->height_clip < 0 ||
+        a->height_clip > HV_ATTN_MAX_HEIGHT_CLIP)
+        return false;
+    if (a->heads > 65535) return false;
+    if (a->batch == 0 || a->queries == 0) return true;
+    return a->q && a->k && a->v && a->token_q && a->token_r && a->token_z && a->token_mask && a->dq_bias &&
+           a->dr_bias && a->dz_bias;
+}
+
+static int attn_classes(const hv_attention* a) { return 2 * (2 * a->coord_clip + 1) + 2 * a->height_clip + 1; }
+
+static int attn_shares(const hv_attention* a) {
+    const int64_t rows = a->batch * a->queries;
+    return (int)(rows < kHistShares ? (rows < 1 ? 1 : rows) : kHistShares);
+}
+
+struct AttnWorkspace {
+    float *p, *ds, *partial;
+    size_t bytes;
+};
+
+static AttnWorkspace attn_workspace(const hv_attention* a, bool back, void* base) {
+    AttnWorkspace w;
+    const size_t pairs = round256((size_t)a->batch * a->heads * a->queries * a->tokens * 4);
+    char* c = static_cast<char*>(base);
+    w.p = reinterpret_cast<float*>(c);
+    w.ds = reinterpret_cast<float*>(c + pairs);
+    w.partial = reinterpret_cast<float*>(c + 2 * pairs);
+    w.bytes = back ? 2 * pairs + (size_t)attn_shares(a) * attn_classes(a) * a->heads * 4 : pairs;
+    return w;
+}
+
+static AttnArgs attn_args(const hv_attention* a) {
+    AttnArgs x = {};
+    x.q = a->q, x.k = a->k, x.v = a->v;
+    for (int i = 0; i < 3; i++) x.qs[i] = a->q_stride[i], x.ks[i] = a->k_stride[i], x.vs[i] = a->v_stride[i];
+    x.tq = a->token_q, x.tr = a->token_r, x.tz = a->token_z, x.mask = a->token_mask;
+    x.tqs = a->token_stride[0], x.trs = a->token_stride[1], x.tzs = a->token_stride[2], x.ms = a->token_stride[3];
+    x.bq = a->dq_bias, x.br = a->dr_bias, x.bz = a->dz_bias;
+    x.t_f32 = a->table_dtype == HV_F32;
+    x.B = a->batch, x.N = a->tokens, x.Nq = a->queries, x.H = a->heads, x.D = a->head_dim;
+    x.clip = a->coord_clip, x.clip_z = a->height_clip, x.scale = a->scale;
+    return x;
+}
+
+}  // namespace hv
+
+using namespace hv;
+
+extern "C" {
+
+int hv_layer_norm_forward(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows,
+                          int width, int dtype, int weight_dtype, float eps, void* sum, void* y, float* mean,
+                          float* rstd, void* stream) {
+    if (rows < 0 || width < 1 || width > kNormMaxWidth || dtype < 0 || dtype > 2) return HV_EINVAL;
+    if (weight_dtype != HV_F32 && weight_dtype != dtype) return HV_EINVAL;
+    if (rows == 0) return HV_OK;
+    if (!x || !weight || !bias || !y || (residual != nullptr) != (sum != nullptr) || !mean != !rstd) return HV_EINVAL;
+    NormShape s;
+    if (!norm_shape(width, dtype, norm_vec(width, dtype, {x, residual, sum, y}), &s)) return HV_EINVAL;
+    NormArgs a = {};
+    a.x = x, a.r = residual, a.w = weight, a.b = bias, a.s = sum, a.y = y, a.mean = mean, a.rstd = rstd;
+    a.rows = rows, a.C = width, a.G = s.G, a.w_f32 = weight_dtype == HV_F32, a.eps = eps;
+    const int grid = norm_grid(s, rows);
+    if (!grid) return HV_ECUDA;
+    return by_type(dtype, [&](auto t) { return launch_norm<decltype(t), false>(a, s, grid, (cudaStream_t)stream); });
+}
+
+int hv_layer_norm_workspace_bytes(int64_t rows, int width, int dtype, size_t* bytes) {
+    NormShape s, t;
+    if (!bytes || rows < 0 || width < 1 || width > kNormMaxWidth || dtype < 0 || dtype > 2) return HV_EINVAL;
+    if (!norm_shape(width, dtype, false, &s) || !norm_shape(width, dtype, true, &t)) return HV_EINVAL;
+    const int64_t per = 148 * kNormBlocksPerSm;
+    *bytes = (size_t)(sm_count() ? (int64_t)sm_count() * kNormBlocksPerSm : per) * 2 * width * 4;
+    return HV_OK;
+}
+
+int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                           const void* dsum, int64_t rows, int width, int dtype, int weight_dtype, void* dx,
+                           void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    if (rows < 0 || width < 1 || width > kNormMaxWidth || dtype < 0 || dtype > 2) return HV_EINVAL;
+    if (weight_dtype != HV_F32 && weight_dtype != dtype) return HV_EINVAL;
+    if (!dweight || !dbias || !workspace || !aligned(workspace, 16)) return HV_EINVAL;
+    if (rows && (!dy || !x || !weight || !mean || !rstd || !dx)) return HV_EINVAL;
+    NormShape s;
+    if (!norm_shape(width, dtype, norm_vec(width, dtype, {dy, x, dsum, dx}), &s)) return HV_EINVAL;
+    const int grid = rows ? norm_grid(s, rows) : 0;
+    if (rows && !grid) return HV_ECUDA;
+    if (workspace_bytes < (size_t)grid * 2 * width * 4) return HV_EINVAL;
+    NormArgs a = {};
+    a.x = x, a.w = weight, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
+    a.dy = dy, a.ds = dsum, a.dx = dx, a.partial = static_cast<float*>(workspace);
+    a.rows = rows, a.C = width, a.G = s.G, a.w_f32 = weight_dtype == HV_F32;
+    const cudaStream_t st = (cudaStream_t)stream;
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (grid) {
+            const int rc = launch_norm<T, true>(a, s, grid, st);
+            if (rc) return rc;
+        }
+        k_norm_reduce<T><<<(2 * width + 31) / 32, 1024, 0, st>>>(a.partial, grid, width, dweight, dbias, a.w_f32);
+        return launched();
+    });
+}
+
+int hv_adamw_step(void* const* params, const void* const* grads, const int64_t* numel, int tensors, int dtype,
+                  void* exp_avg, void* exp_avg_sq, float* avg_scale, float* sq_scale, int state_bits, float beta1,
+                  float one_minus_beta1, float beta2, float one_minus_beta2, float eps, float decay, float step_size,
+                  float inv_root_correction2, uint32_t key, void* stream) {
+    if (tensors < 0 || dtype < 0 || dtype > 2 || (state_bits != 8 && state_bits != 32)) return HV_EINVAL;
+    if (tensors == 0) return HV_OK;
+    const bool small = state_bits == 8;
+    if (!params || !grads || !numel || !exp_avg || !exp_avg_sq || (small && (!avg_scale || !sq_scale))) return HV_EINVAL;
+    if (!aligned(exp_avg, 16) || !aligned(exp_avg_sq, 16)) return HV_EINVAL;
+    for (int i = 0; i < tensors; i++) {
+        if (numel[i] < 0 || (numel[i] && (!params[i] || !grads[i]))) return HV_EINVAL;
+        if (!aligned(params[i], elem_bytes(dtype)) || !aligned(grads[i], elem_bytes(dtype))) return HV_EINVAL;
+        if (numel[i] > ((int64_t)1 << 38)) return HV_EINVAL;
+    }
+    const AdamScalars sc = {beta1, one_minus_beta1, beta2, one_minus_beta2, eps, decay, step_size, inv_root_correction2,
+                            key};
+    // a launch's table holds up to CAP tensors and 2^30 units; the small table keeps the
+    // argument block of a usual step at 4 KB
+    auto run = [&](auto t, auto cap) -> int {
+        using T = decltype(t);
+        constexpr int CAP = decltype(cap)::value;
+        int64_t unit0 = 0;
+        for (int i = 0; i < tensors;) {
+            AdamTable<CAP> tab;
+            int n = 0;
+            int64_t units = 0;
+            for (; i < tensors && n < CAP; i++) {
+                const int64_t u = (numel[i] + kAdamBlock - 1) / kAdamBlock;
+                if (!u) continue;
+                if (units + u > (1 << 30) && n) break;
+                tab.p[n] = params[i], tab.g[n] = grads[i], tab.n[n] = numel[i], tab.first[n] = (int32_t)units;
+                units += u, n++;
+            }
+            if (!n) break;
+            tab.first[n] = (int32_t)units, tab.tensors = n;
+            const unsigned grid = (unsigned)((units + kAdamWarps - 1) / kAdamWarps);
+            if (small)
+                k_adamw<T, true, CAP><<<grid, kAdamWarps * 32, 0, (cudaStream_t)stream>>>(tab, exp_avg, exp_avg_sq, avg_scale,
+                                                                                         sq_scale, unit0, sc);
+            else
+                k_adamw<T, false, CAP><<<grid, kAdamWarps * 32, 0, (cudaStream_t)stream>>>(tab, exp_avg, exp_avg_sq, nullptr,
+                                                                                          nullptr, unit0, sc);
+            const int rc = launched();
+            if (rc) return rc;
+            unit0 += units;
+        }
+        return HV_OK;
+    };
+    return by_type(dtype, [&](auto t) {
+        return tensors <= 128 ? run(t, std::integral_constant<int, 128>()) : run(t, std::integral_constant<int, 1024>());
+    });
+}
+
+int hv_adamw_state_values(const uint8_t* codes, const float* scale, int64_t count, int second, float* out, void* stream) {
+    if (count < 0 || count % kAdamBlock) return HV_EINVAL;
+    if (count == 0) return HV_OK;
+    if (!codes || !scale || !out || !aligned(codes, 4) || !aligned(out, 16)) return HV_EINVAL;
+    const int64_t words = count / 4, grid = (words + 255) / 256;
+    if (grid > 0x7fffffff) return HV_EINVAL;
+    const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
+    if (second)
+        k_adamw_values<true><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(c, scale, words, out);
+    else
+        k_adamw_values<false><<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(c, scale, words, out);
+    return launched();
+}
+
+int hv_relative_attention_sizes(const hv_attention* a, size_t* saved_bytes, size_t* forward_bytes, size_t* backward_bytes) {
+    if (!attn_ok(a) || !saved_bytes || !forward_bytes || !backward_bytes) return HV_EINVAL;
+    *saved_bytes = 0;
+    *forward_bytes = attn_workspace(a, false, nullptr).bytes;
+    *backward_bytes = attn_workspace(a, true, nullptr).bytes;
+    return HV_OK;
+}
+
+int hv_relative_attention_forward(const hv_attention* a, void* out, void* saved, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    (void)saved;
+    if (!attn_ok(a)) return HV_EINVAL;
+    if (a->batch == 0 || a->queries == 0) return HV_OK;
+    const AttnWorkspace w = attn_workspace(a, false, workspace);
+    if (!out || !workspace || !aligned(workspace, 256) || workspace_bytes < w.bytes) return HV_EINVAL;
+    AttnArgs x = attn_args(a);
+    x.out = out, x.p = w.p;
+    const int64_t grid = (x.B * x.H * x.Nq + 3) / 4;
+    if (grid > 0x7fffffff) return HV_EINVAL;
+    return by_type(a->dtype, [&](auto t) {
+        k_attn_row<decltype(t), false><<<(unsigned)grid, 128, 0, (cudaStream_t)stream>>>(x);
+        return launched();
+    });
+}
+
+int hv_relative_attention_backward(const hv_attention* a, const void* dout, const int64_t* dout_stride, const void* saved,
+                                   void* dq, void* dk, void* dv, const int64_t* dq_stride, const int64_t* dkv_stride,
+                                   void* ddq_bias, void* ddr_bias, void* ddz_bias, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    (void)saved;
+    if (!attn_ok(a) || !ddq_bias || !ddr_bias || !ddz_bias) return HV_EINVAL;
+    const bool empty = a->batch == 0 || a->queries == 0;
+    if (a->batch && a->tokens && (!dk || !dv || !dkv_stride)) return HV_EINVAL;
+    if (!empty && (!dout || !dout_stride || !dq || !dq_stride)) return HV_EINVAL;
+    const AttnWorkspace w = attn_workspace(a, true, workspace);
+    if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.bytes) return HV_EINVAL;
+    AttnArgs x = attn_args(a);
+    x.dout = dout, x.dq = dq, x.dk = dk, x.dv = dv, x.p = w.p, x.ds = w.ds, x.partial = w.partial;
+    for (int i = 0; i < 3; i++) {
+        x.os[i] = dout_stride ? dout_stride[i] : 0, x.gs[i] = dq_stride ? dq_stride[i] : 0;
+        x.gks[i] = dkv_stride ? dkv_stride[i] : 0;
+    }
+    const int64_t rows = (x.B * x.H * x.Nq + 3) / 4, keys = (x.B * x.H * x.N + 3) / 4;
+    if (rows > 0x7fffffff || keys > 0x7fffffff) return HV_EINVAL;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const int W = 2 * x.clip + 1, classes = attn_classes(a), shares = attn_shares(a);
+    return by_type(a->dtype, [&](auto t) {
+        using T = decltype(t);
+        int rc;
+        if (rows) {
+            k_attn_row<T, true><<<(unsigned)rows, 128, 0, st>>>(x);
+            if ((rc = launched())) return rc;
+        }
+        if (keys) {
+            k_attn_key<T><<<(unsigned)keys, 128, 0, st>>>(x);
+            if ((rc = launched())) return rc;
+        }
+        k_attn_table<<<dim3(shares, x.H), 32, classes * 128, st>>>(x);
+        if ((rc = launched())) return rc;
+        k_attn_table_sum<T><<<(classes * x.H + 3) / 4, 128, 0, st>>>(x.partial, shares, W, classes, x.H, ddq_bias, ddr_bias,
+                                                                    ddz_bias, x.t_f32);
+        return launched();
+    });
+}
+
+}  // extern "C"

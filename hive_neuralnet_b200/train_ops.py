@@ -1,0 +1,492 @@
+"""Training operators on the sm_100a kernels: attention with a learned
+(dq, dr, dz) offset bias per head, layer norm with the residual added first,
+and an AdamW step over many tensors at once.
+
+Each operator is there twice: as a forward / backward pair on plain tensors
+(``relative_attention_forward`` / ``relative_attention_backward``,
+``layer_norm_forward`` / ``layer_norm_backward``), and under autograd
+(:func:`relative_attention`, :func:`relative_attention_packed`,
+:func:`layer_norm`).  :class:`AdamW` holds the moments of a parameter list;
+:func:`adamw_step` is one step on tensors of the caller's.
+
+Activations are float32, float16 or bfloat16; arithmetic, statistics and sums
+are float32.  Everything runs on the current stream of the tensors' device,
+without synchronising, and gives the same bits on every run.  There is no CPU
+path: arguments of another device, type or shape raise ``ValueError``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_HEAD_DIM = 64
+MAX_COORD_CLIP, MAX_HEIGHT_CLIP = 16, 4
+MAX_NORM_WIDTH = 8192
+STATE_BLOCK = 256
+
+
+def _dtype(t: torch.Tensor, name: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None or not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA float32, float16 or bfloat16 tensor")
+    return code
+
+
+class _on:
+    """The tensors' device made current, where it is not, for the library call."""
+
+    def __init__(self, dev):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _stream(dev) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+# ---------------------------------------------------------------------------
+# relative attention
+# ---------------------------------------------------------------------------
+def _heads(t, name, b, n, h, d, like):
+    """A [b, n, h, d] operand of ``like``'s type with the head's values
+    contiguous (copied if they are not), and its (batch, token, head) strides."""
+    if t.shape != (b, n, h, d) or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name}: expected {like.dtype} [{b}, {n}, {h}, {d}] on {like.device}, got {t.dtype} "
+                         f"{list(t.shape)} on {t.device}")
+    st = t.stride()
+    if st[3] != 1 and d > 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, st
+
+
+def _tokens(t, name, b, n, dev):
+    if t.shape != (b, n) or t.device != dev or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name}: expected int32 or int64 [{b}, {n}] on {dev}")
+    if t.dtype != torch.int32:
+        t = t.clamp(-(1 << 19), 1 << 19).to(torch.int32)  # the range the operator clamps to
+    return t if n < 2 or t.stride(1) == 1 else t.contiguous()
+
+
+class _Problem:
+    """Checked arguments of one call, kept alive with the struct that points at them."""
+
+    def __init__(self, q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, scale):
+        dtype = _dtype(q, "q")
+        if q.dim() != 4 or k.dim() != 4:
+            raise ValueError("q, k, v: expected [batch, tokens, heads, head_dim]")
+        b, nq, h, d = q.shape
+        n = k.shape[1]
+        dev = q.device
+        if nq > n:
+            raise ValueError(f"q has {nq} tokens, k has {n}: the queries are the first tokens")
+        if not 1 <= d <= MAX_HEAD_DIM or h < 1 or h > 65535:
+            raise ValueError(f"head_dim: 1 to {MAX_HEAD_DIM}, heads: 1 to 65535 (got {d}, {h})")
+        q, qs = _heads(q, "q", b, nq, h, d, q)
+        k, ks = _heads(k, "k", b, n, h, d, q)
+        v, vs = _heads(v, "v", b, n, h, d, q)
+        tq, tr, tz = (_tokens(t, name, b, n, dev) for t, name in
+                      ((token_q, "token_q"), (token_r, "token_r"), (token_z, "token_z")))
+        m = token_mask
+        if m.shape != (b, n) or m.device != dev or m.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"token_mask: expected bool or uint8 [{b}, {n}] on {dev}")
+        if n > 1 and m.stride(1) != 1:
+            m = m.contiguous()
+        clips = []
+        for t, name, most in ((dq_bias, "dq_bias", MAX_COORD_CLIP), (dr_bias, "dr_bias", MAX_COORD_CLIP),
+                              (dz_bias, "dz_bias", MAX_HEIGHT_CLIP)):
+            if t.dim() != 2 or t.shape[1] != h or t.shape[0] % 2 == 0 or t.shape[0] > 2 * most + 1 or t.device != dev:
+                raise ValueError(f"{name}: expected [2 clip + 1, {h}] with clip at most {most} on {dev}")
+            clips.append(t.shape[0] // 2)
+        if clips[0] != clips[1]:
+            raise ValueError("dq_bias and dr_bias have different clips")
+        tables = [t.contiguous() for t in (dq_bias, dr_bias, dz_bias)]
+        td = tables[0].dtype
+        if td not in (torch.float32, q.dtype) or any(t.dtype != td for t in tables):
+            raise ValueError("bias tables: expected float32 or the type of q, all three alike")
+        self.keep = (q, k, v, tq, tr, tz, m, *tables)
+        self.q, self.table_dtype, self.table_shapes = q, td, [t.shape for t in tables]
+        self.dims, self.dev, self.self_attention = (b, n, nq, h, d), dev, nq == n
+        i3, i4 = C.c_int64 * 3, C.c_int64 * 4
+        self.arg = _lib.HvAttention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), i3(*qs[:3]), i3(*ks[:3]), i3(*vs[:3]), tq.data_ptr(),
+            tr.data_ptr(), tz.data_ptr(), m.data_ptr(),
+            i4(tq.stride(0), tr.stride(0), tz.stride(0), m.stride(0)), *(t.data_ptr() for t in tables), b, n, nq, h, d,
+            clips[0], clips[2], dtype, _DTYPES[td], float(d ** -0.5 if scale is None else scale))
+
+    def sizes(self):
+        s = (C.c_size_t * 3)()
+        at = C.addressof(s)
+        _lib.check(_lib.load().hv_relative_attention_sizes(self.arg, at, at + 8, at + 16), "relative_attention_sizes")
+        return s
+
+    def buffer(self, nbytes):
+        return torch.empty((nbytes,), dtype=torch.uint8, device=self.dev) if nbytes else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def relative_attention_forward(q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, *,
+                               scale=None, save=False):
+    """Attention over padded tokens with a learned bias per head for the clipped
+    (dq, dr, dz) offset of key from query; returns ``(out, saved)``.
+
+    q [B, Nq, H, D]: the first Nq of the N tokens (Nq = N for all, 1 for the CLS
+    row alone); k, v [B, N, H, D]; any batch, token and head strides, so the
+    views of a fused projection [B, N, 3, H, D] go in as they are.  token_q /
+    token_r / token_z [B, N] (clamped to +-2^19) and token_mask [B, N] may be
+    expanded over the batch.  dq_bias, dr_bias [2 clip + 1, H], dz_bias
+    [2 height_clip + 1, H].  scale defaults to D ** -0.5.
+
+    A masked token neither attends nor is attended to: its output row is zero
+    and what it holds is never used.  ``saved`` goes to
+    :func:`relative_attention_backward`; without ``save`` it is None.
+    """
+    p = _Problem(q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, scale)
+    b, n, nq, h, d = p.dims
+    out = torch.empty((b, nq, h, d), dtype=q.dtype, device=p.dev)
+    with _on(p.dev):
+        sizes = p.sizes()
+        saved, ws = p.buffer(sizes[0] if save else 0), p.buffer(sizes[1])
+        _lib.check(_lib.load().hv_relative_attention_forward(p.arg, out.data_ptr(), _ptr(saved), _ptr(ws), sizes[1],
+                                                             _stream(p.dev)), "relative_attention_forward")
+    return out, saved
+
+
+def relative_attention_backward(dout, q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias,
+                                saved, *, scale=None):
+    """Gradients ``(dq, dk, dv, ddq_bias, ddr_bias, ddz_bias)`` of
+    :func:`relative_attention_forward` for ``dout`` [B, Nq, H, D]; the
+    probabilities are recomputed.  With Nq = N the first three are views of one
+    [B, N, 3, H, D] tensor."""
+    p = _Problem(q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, scale)
+    return _backward(p, dout, saved)[0]
+
+
+def _backward(p, dout, saved):
+    b, n, nq, h, d = p.dims
+    dout, gs = _heads(dout, "dout", b, nq, h, d, p.q)
+    if p.self_attention:
+        packed = torch.empty((b, n, 3, h, d), dtype=p.q.dtype, device=p.dev)
+        dq, dk, dv = packed.unbind(2)
+    else:
+        packed = torch.empty((b, n, 2, h, d), dtype=p.q.dtype, device=p.dev)
+        dk, dv = packed.unbind(2)
+        dq = torch.empty((b, nq, h, d), dtype=p.q.dtype, device=p.dev)
+    tables = [torch.empty(s, dtype=p.table_dtype, device=p.dev) for s in p.table_shapes]
+    i3 = C.c_int64 * 3
+    with _on(p.dev):
+        sizes = p.sizes()
+        if saved is None and sizes[0]:
+            raise ValueError("saved: the forward pass was run without save=True")
+        if saved is not None and saved.numel() != sizes[0]:
+            raise ValueError("saved: not of a forward pass of this shape")
+        ws = p.buffer(sizes[2])
+        gst, dst = i3(*gs[:3]), i3(*dk.stride()[:3])
+        dqs = i3(*dq.stride()[:3])
+        _lib.check(_lib.load().hv_relative_attention_backward(
+            p.arg, dout.data_ptr(), C.addressof(gst), _ptr(saved), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            C.addressof(dqs), C.addressof(dst), *(t.data_ptr() for t in tables), _ptr(ws), sizes[2], _stream(p.dev)),
+            "relative_attention_backward")
+    return (dq, dk, dv, *tables), packed
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scale, q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias):
+        args = (q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias)
+        out, saved = relative_attention_forward(*args, scale=scale, save=True)
+        ctx.scale, ctx.has_saved = scale, saved is not None
+        ctx.save_for_backward(*args, *([saved] if ctx.has_saved else []))
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        t = ctx.saved_tensors
+        p = _Problem(*t[:10], ctx.scale)
+        (dq, dk, dv, *tables), _ = _backward(p, dout, t[10] if ctx.has_saved else None)
+        return None, dq, dk, dv, None, None, None, None, *tables
+
+
+def relative_attention(q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, *, scale=None):
+    """:func:`relative_attention_forward` under autograd."""
+    return _Attention.apply(scale, q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias)
+
+
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scale, qkv, *rest):
+        out, saved = relative_attention_forward(*qkv.unbind(2), *rest, scale=scale, save=True)
+        ctx.scale, ctx.has_saved = scale, saved is not None
+        ctx.save_for_backward(qkv, *rest, *([saved] if ctx.has_saved else []))
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, *t = ctx.saved_tensors
+        p = _Problem(*qkv.unbind(2), *t[:7], ctx.scale)
+        grads, packed = _backward(p, dout, t[7] if ctx.has_saved else None)
+        return None, packed, None, None, None, None, *grads[3:]
+
+
+def relative_attention_packed(qkv, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, *, scale=None):
+    """:func:`relative_attention` on a fused projection qkv [B, N, 3, H, D]; its
+    gradient comes back as one tensor of that shape."""
+    if qkv.dim() != 5 or qkv.shape[2] != 3:
+        raise ValueError("qkv: expected [batch, tokens, 3, heads, head_dim]")
+    return _PackedAttention.apply(scale, qkv, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias)
+
+
+# ---------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------
+def _rows(t, name, like):
+    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name}: expected {like.dtype} {list(like.shape)} on {like.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _norm_params(x, weight, bias):
+    dtype = _dtype(x, "x")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_WIDTH:
+        raise ValueError(f"x: the last axis must hold 1 to {MAX_NORM_WIDTH} values")
+    w = x.shape[-1]
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.shape != (w,) or t.device != x.device or t.dtype not in (torch.float32, x.dtype) or t.dtype != weight.dtype:
+            raise ValueError(f"{name}: expected [{w}], float32 or {x.dtype}, on {x.device}")
+    return dtype, w, x.numel() // w
+
+
+def layer_norm_forward(x, weight, bias, eps=1e-5, residual=None):
+    """Layer norm over the last axis (1 to 8192 values) of x, or of x + residual;
+    returns ``(y, s, mean, rstd)``: s is what was normalised (x itself, or the
+    sum in x's type), mean and rstd float32 over the leading axes.  weight and
+    bias are float32 or of x's type."""
+    dtype, w, rows = _norm_params(x, weight, bias)
+    x = x if x.is_contiguous() else x.contiguous()
+    dev = x.device
+    s = x
+    if residual is not None:
+        residual = _rows(residual, "residual", x)
+        s = torch.empty_like(x)
+    y = torch.empty_like(x)
+    stats = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=dev)
+    mean, rstd = stats.unbind(0)
+    weight, bias = weight.contiguous(), bias.contiguous()
+    with _on(dev):
+        _lib.check(_lib.load().hv_layer_norm_forward(
+            x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), rows, w, dtype, _DTYPES[weight.dtype],
+            eps, None if residual is None else s.data_ptr(), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+            _stream(dev)), "layer_norm_forward")
+    return y, s, mean, rstd
+
+
+def layer_norm_backward(dy, s, weight, mean, rstd, dsum=None):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`layer_norm_forward` for dy,
+    where s, mean and rstd are what it returned.  dsum: a gradient that reaches
+    s by another way (the residual stream), added into dx; dx is the gradient of
+    x and of the residual."""
+    dtype, w, rows = _norm_params(s, weight, None)
+    dy = _rows(dy, "dy", s)
+    if dsum is not None:
+        dsum = _rows(dsum, "dsum", s)
+    dev = s.device
+    s, weight = s.contiguous(), weight.contiguous()
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype != torch.float32 or t.shape != s.shape[:-1] or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous float32 {list(s.shape[:-1])} on {dev}")
+    dx = torch.empty_like(s)
+    dw, db = torch.empty((2, w), dtype=weight.dtype, device=dev).unbind(0)
+    lib = _lib.load()
+    with _on(dev):
+        need = C.c_size_t(0)
+        _lib.check(lib.hv_layer_norm_workspace_bytes(rows, w, dtype, C.addressof(need)), "layer_norm_workspace_bytes")
+        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
+        _lib.check(lib.hv_layer_norm_backward(
+            dy.data_ptr(), s.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(dsum), rows, w,
+            dtype, _DTYPES[weight.dtype], dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need.value,
+            _stream(dev)), "layer_norm_backward")
+    return dx, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, residual):
+        y, s, mean, rstd = layer_norm_forward(x, weight, bias, eps, residual)
+        ctx.residual = residual is not None
+        ctx.save_for_backward(s, weight, mean, rstd)
+        ctx.set_materialize_grads(False)
+        return (y, s) if ctx.residual else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dsum=None):
+        s, weight, mean, rstd = ctx.saved_tensors
+        if dy is None:  # only the sum was used
+            return dsum, None, None, None, dsum if ctx.residual else None
+        dx, dw, db = layer_norm_backward(dy, s, weight, mean, rstd, dsum)
+        return dx, dw, db, None, dx if ctx.residual else None
+
+
+def layer_norm(x, weight, bias, eps=1e-5, residual=None):
+    """:func:`layer_norm_forward` under autograd: y, or ``(y, x + residual)``."""
+    return _LayerNorm.apply(x, weight, bias, eps, residual)
+
+
+# ---------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------
+def state_size(params) -> int:
+    """Values in each flat moment of a parameter list: a tensor's part begins at
+    the next multiple of 256 after the one before."""
+    return sum(-(-p.numel() // STATE_BLOCK) * STATE_BLOCK for p in params)
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+               scales=None, seed=0):
+    """One AdamW step (the ``step``-th, from 1) over all of ``params``, in place.
+
+    params and grads: lists of dense CUDA tensors of one type (float32, float16
+    or bfloat16; the update is computed in float32 and rounded to nearest once).
+    exp_avg, exp_avg_sq: flat states of :func:`state_size` values, float32; or
+    uint8 with ``scales`` = (avg_scale, sq_scale), float32, one for each 256
+    values, rounded stochastically by a hash of position, step and seed.  A
+    non-finite gradient makes its parameter (and with 8-bit states the moments
+    of its 256 values) non-finite.
+    """
+    count = len(params)
+    if count != len(grads):
+        raise ValueError(f"{count} params, {len(grads)} grads")
+    if step < 1:
+        raise ValueError("step counts from 1")
+    if count == 0:
+        return
+    first = params[0]
+    dtype, dev, kind = _dtype(first, "params[0]"), first.device, first.dtype
+    total, numel, pp, gp, keep = 0, [], [], [], []
+    for i, (p, g) in enumerate(zip(params, grads)):
+        if p.dtype is not kind or g.dtype is not kind or p.device != dev or g.device != dev or g.shape != p.shape:
+            raise ValueError(f"params[{i}], grads[{i}]: expected {kind} of one shape on {dev}")
+        if not p.is_contiguous():
+            raise ValueError(f"params[{i}]: expected a contiguous tensor")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            keep.append(g)
+        n = p.numel()
+        total += -(-n // STATE_BLOCK) * STATE_BLOCK
+        numel.append(n)
+        pp.append(p.data_ptr())
+        gp.append(g.data_ptr())
+    want = torch.float32 if scales is None else torch.uint8
+    states = [(exp_avg, "exp_avg", want, total), (exp_avg_sq, "exp_avg_sq", want, total)]
+    if scales is not None:
+        states += [(scales[0], "scales[0]", torch.float32, total // STATE_BLOCK),
+                   (scales[1], "scales[1]", torch.float32, total // STATE_BLOCK)]
+    for t, name, dt, size in states:
+        if t.dtype is not dt or t.numel() != size or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous {dt} of {size} values on {dev}")
+    (b1, b2), seed, step = betas, int(seed), int(step)
+    key = (seed * 0x6A09E667 + step * 0xBB67AE85) & 0xFFFFFFFF
+    ptrs, sizes = C.c_void_p * count, C.c_int64 * count
+    pa, ga, na = ptrs(*pp), ptrs(*gp), sizes(*numel)
+    with _on(dev):
+        _lib.check(_lib.load().hv_adamw_step(
+            C.addressof(pa), C.addressof(ga), C.addressof(na), count, dtype, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+            None if scales is None else scales[0].data_ptr(), None if scales is None else scales[1].data_ptr(),
+            32 if scales is None else 8, b1, 1 - b1, b2, 1 - b2, eps, 1 - lr * weight_decay, lr / (1 - b1 ** step),
+            1 / math.sqrt(1 - b2 ** step), key, _stream(dev)), "adamw_step")
+
+
+def _state_values(codes, scale, second):
+    if codes.dtype != torch.uint8 or scale.dtype != torch.float32 or not codes.is_cuda or scale.device != codes.device:
+        raise ValueError("codes: expected CUDA uint8, scale: float32 on the same device")
+    if codes.numel() != scale.numel() * STATE_BLOCK or not codes.is_contiguous() or not scale.is_contiguous():
+        raise ValueError(f"expected contiguous codes, {STATE_BLOCK} for each scale")
+    out = torch.empty((codes.numel(),), dtype=torch.float32, device=codes.device)
+    with _on(codes.device):
+        _lib.check(_lib.load().hv_adamw_state_values(codes.data_ptr(), scale.data_ptr(), codes.numel(), second,
+                                                     out.data_ptr(), _stream(codes.device)), "adamw_state_values")
+    return out
+
+
+def exp_avg_values(codes, scale):
+    """The float32 first moments that 8-bit states stand for."""
+    return _state_values(codes, scale, 0)
+
+
+def exp_avg_sq_values(codes, scale):
+    """The float32 second moments that 8-bit states stand for (the codes hold their roots)."""
+    return _state_values(codes, scale, 1)
+
+
+class AdamW:
+    """AdamW over a list of parameters: every tensor in one launch a step.
+
+    ``state_bits`` 32 keeps the moments in float32, 8 in one byte each with a
+    float32 scale for 256 values.  All parameters have a gradient when
+    :meth:`step` is called; lr, betas, eps and weight_decay may be changed
+    between steps.  ``state_dict`` / ``load_state_dict`` carry the moments.
+    """
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
+        self.params = [p for p in params]
+        if not self.params:
+            raise ValueError("no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits: 8 or 32")
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("lr, eps and weight_decay must not be negative, betas in [0, 1)")
+        self.lr, self.betas, self.eps, self.weight_decay, self.seed = lr, tuple(betas), eps, weight_decay, int(seed)
+        self.state_bits, self.steps = state_bits, 0
+        n, dev = state_size(self.params), self.params[0].device
+        dt = torch.float32 if state_bits == 32 else torch.uint8
+        self.exp_avg, self.exp_avg_sq = (torch.zeros(n, dtype=dt, device=dev) for _ in range(2))
+        self.scales = None if state_bits == 32 else tuple(torch.zeros(n // STATE_BLOCK, device=dev) for _ in range(2))
+
+    @torch.no_grad()
+    def step(self) -> None:
+        grads = [p.grad for p in self.params]
+        if any(g is None for g in grads):
+            raise ValueError("every parameter needs a gradient")
+        adamw_step(self.params, grads, self.exp_avg, self.exp_avg_sq, step=self.steps + 1, lr=self.lr,
+                   betas=self.betas, eps=self.eps, weight_decay=self.weight_decay, scales=self.scales, seed=self.seed)
+        self.steps += 1
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        for p in self.params:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+
+    def state_dict(self) -> dict:
+        return dict(steps=self.steps, state_bits=self.state_bits, seed=self.seed, exp_avg=self.exp_avg,
+                    exp_avg_sq=self.exp_avg_sq, scales=self.scales)
+
+    def load_state_dict(self, state: dict) -> None:
+        if state["state_bits"] != self.state_bits or state["exp_avg"].shape != self.exp_avg.shape:
+            raise ValueError("the state is of other parameters or state_bits")
+        self.steps, self.seed = state["steps"], state["seed"]
+        self.exp_avg.copy_(state["exp_avg"])
+        self.exp_avg_sq.copy_(state["exp_avg_sq"])
+        if self.scales is not None:
+            for mine, theirs in zip(self.scales, state["scales"]):
+                mine.copy_(theirs)

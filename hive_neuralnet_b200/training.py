@@ -4,15 +4,22 @@
 ``FNNTrainer._build_forward_batch`` (hive_fnn/fnn_trainer.py:531-580): root
 features, every successor's features, the successor -> root map and the
 action counts of a replay batch, ready for a differentiable torch forward of
-``HiveFNN`` (training keeps autograd in torch; only the inputs come from the
-kernels).  ``build_hybrid_forward_batch`` adds the hybrid network's piece
+``HiveFNN``.  ``build_hybrid_forward_batch`` adds the hybrid network's piece
 tokens and per-move features (the replay buffer's cached bundle,
 hive_fnn/fnn_replay_buffer.py:405-466).
+
+``hybrid_forward`` and ``hybrid_train_step`` train the hybrid network with its
+attention, norms and optimizer on the kernels of :mod:`.train_ops`; the module's
+own torch forward computes the same.
 """
 from __future__ import annotations
 
+from dataclasses import replace
+
 import torch
 
+from . import train_ops
+from .fnn import MAX_LEGAL
 from .hive_gpu import load_extension
 from .hybrid import HybridPieceTensorBatch
 
@@ -60,3 +67,83 @@ def build_hybrid_forward_batch(state_bytes: torch.Tensor, batch_size: int):
             else root_features[:0])
     pb = HybridPieceTensorBatch(tf, tq, tr, tz, tm, gf, tm.sum(dim=1, dtype=torch.int32))
     return root_features, succ, action_to_root, num_actions, pb, move_features[valid]
+
+
+# ---------------------------------------------------------------------------
+# a training step on the kernels
+# ---------------------------------------------------------------------------
+def _norm(x: torch.Tensor, m: torch.nn.LayerNorm, residual: torch.Tensor | None = None):
+    return train_ops.layer_norm(x, m.weight, m.bias, m.eps, residual)
+
+
+def trunk_forward(trunk, pb: HybridPieceTensorBatch) -> torch.Tensor:
+    """``HybridRelativeTransformerTrunk.forward`` under autograd with the attention
+    and the norms on the training kernels (:mod:`.train_ops`): the same summary
+    [B, H] and the same gradients.  Any preset.  Masked tokens take no part in
+    the attention, so their rows need no clearing between the blocks, and the
+    last block attends from the CLS token alone."""
+    b = pb.token_features.shape[0]
+    tokens = trunk.token_proj(pb.token_features)
+    s = torch.cat([trunk.cls_token.expand(b, -1, -1).to(tokens.dtype), tokens], dim=1)
+    n = s.shape[1]
+    zero = torch.zeros((b, 1), dtype=torch.int32, device=s.device)
+    where = [torch.cat([zero, t.to(torch.int32)], dim=1) for t in (pb.token_q, pb.token_r, pb.token_z)]
+    where.append(torch.cat([torch.ones((b, 1), dtype=torch.bool, device=s.device), pb.token_mask.bool()], dim=1))
+    out = None  # the branch output not yet added to the residual stream s
+    for i, layer in enumerate(trunk.layers):
+        a = layer.attn
+        if out is None:
+            y = _norm(s, layer.norm1)
+        else:
+            y, s = _norm(out.to(s.dtype), layer.norm1, s)
+        qkv = a.qkv(y).view(b, n, 3, a.num_heads, a.head_dim)
+        tables = (a.dq_bias.weight, a.dr_bias.weight, a.dz_bias.weight)
+        if i + 1 < len(trunk.layers):
+            o = train_ops.relative_attention_packed(qkv, *where, *tables, scale=a.scale)
+        else:
+            q, k, v = qkv.unbind(2)
+            o = train_ops.relative_attention(q[:, :1], k, v, *where, *tables, scale=a.scale)
+            s = s[:, :1].contiguous()
+        y, s = _norm(a.out_proj(o.flatten(2)).to(s.dtype), layer.norm2, s)
+        out = layer.ffn(y)
+    y, _ = _norm(out.to(s.dtype), trunk.norm, s) if out is not None else (_norm(s[:, :1].contiguous(), trunk.norm), s)
+    return y[:, 0]
+
+
+def _encode(fnn, features: torch.Tensor) -> torch.Tensor:
+    return fnn.fc2(_norm(torch.sigmoid(fnn.fc1(features)), fnn.ln1))
+
+
+def hybrid_forward(net, root_features, successor_features, action_to_root, num_actions, piece_batch, move_features):
+    """``HiveHybridGNN.forward`` on the training kernels: (logits [N], values [B, 1])."""
+    root_emb = _encode(net.fnn, root_features)
+    g = trunk_forward(net.graph_trunk, piece_batch)
+    if action_to_root.shape[0] == 0:
+        logits = root_features.new_zeros((0,))
+    else:
+        logits = net.score_hybrid_actions(root_emb[action_to_root], g[action_to_root],
+                                          _encode(net.fnn, successor_features), move_features)
+    return logits, torch.tanh(net.value_head(torch.cat([root_emb, g, piece_batch.global_features], dim=1)))
+
+
+def hybrid_train_step(net, optimizer, batch, policy_target: torch.Tensor, value_target: torch.Tensor,
+                      value_weight: float = 1.0):
+    """One step on a batch of :func:`build_hybrid_forward_batch`: forward, cross
+    entropy of the legal moves' softmax against ``policy_target`` [N] plus the
+    squared error of the values against ``value_target`` [B], backward, and
+    ``optimizer.step()`` (:class:`.train_ops.AdamW`).  Returns the two losses."""
+    _, _, action_to_root, num_actions, piece_batch, _ = batch
+    use = net.config.node_feat_dim
+    if piece_batch.token_features.shape[-1] != use:
+        piece_batch = replace(piece_batch, token_features=piece_batch.token_features[..., :use])
+    optimizer.zero_grad()
+    logits, values = hybrid_forward(net, *batch[:4], piece_batch, batch[5])
+    b = num_actions.shape[0]
+    slot = torch.arange(logits.shape[0], device=logits.device) - (num_actions.cumsum(0) - num_actions)[action_to_root]
+    dense = logits.new_full((b, MAX_LEGAL), float("-inf")).index_put((action_to_root, slot), logits)
+    log_p = torch.log_softmax(dense.float(), dim=1)[action_to_root, slot]
+    policy_loss = -(policy_target * log_p).sum() / b
+    value_loss = (values.squeeze(1).float() - value_target).square().mean()
+    (policy_loss + value_weight * value_loss).backward()
+    optimizer.step()
+    return policy_loss.detach(), value_loss.detach()

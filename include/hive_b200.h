@@ -23,6 +23,7 @@
 #ifndef HIVE_B200_H
 #define HIVE_B200_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -439,6 +440,98 @@ int hv_legal_moves_to_actions(const uint8_t* states, const uint8_t* moves, const
  * the spirit of hive_gpu/endgame_generator.py:284-289 (random playouts). */
 int hv_generate_positions(uint64_t seed, int64_t first_game, int64_t count, int max_ply,
                           int expansion_mask, uint8_t* states, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Training operators (csrc/hv_train.cu).  The reference trains its hybrid
+ * network through torch autograd (hive_fnn_transformer/fnn_transformer_net.py);
+ * these have no binding there.  dtype: the type of the activations (or of the
+ * parameters, for AdamW); arithmetic, statistics and sums are fp32 throughout.
+ * Results do not depend on the order in which blocks run.
+ * ------------------------------------------------------------------------- */
+enum hv_dtype { HV_F32 = 0, HV_F16 = 1, HV_BF16 = 2 };
+
+/* Layer norm of `rows` contiguous rows of `width` (1 .. 8192) values.  With a
+ * residual, sum = x + residual (in dtype) is written and normalised; both NULL
+ * otherwise.  weight, bias: weight_dtype (fp32, or dtype).  mean, rstd: [rows]
+ * fp32 for the backward pass, or both NULL. */
+int hv_layer_norm_forward(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows,
+                          int width, int dtype, int weight_dtype, float eps, void* sum, void* y, float* mean,
+                          float* rstd, void* stream);
+
+/* Its backward pass; x is what was normalised (the sum, with a residual).
+ * dsum (NULL: none) is a further gradient of x, added into dx.  dweight and
+ * dbias are written in weight_dtype (zeros for no rows).  workspace: 16-byte
+ * aligned, hv_layer_norm_workspace_bytes bytes on the current device. */
+int hv_layer_norm_workspace_bytes(int64_t rows, int width, int dtype, size_t* bytes);
+int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                           const void* dsum, int64_t rows, int width, int dtype, int weight_dtype, void* dx,
+                           void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step over `tensors` dense tensors (params[i], grads[i]: numel[i]
+ * values of dtype; the pointer and size arrays are host memory and are read
+ * during the call only).  The moments are flat: a tensor's part begins at the
+ * next multiple of 256 values after the one before.  state_bits 32: exp_avg
+ * and exp_avg_sq are fp32; 8: one byte a value, with a scale for each 256
+ * (avg_scale, sq_scale).  16-byte aligned.
+ *   m = beta1 m + one_minus_beta1 g;  v = beta2 v + one_minus_beta2 g^2
+ *   p = p decay - step_size m / (sqrt(v) inv_root_correction2 + eps)
+ * with decay = 1 - lr wd, step_size = lr / (1 - beta1^t),
+ * inv_root_correction2 = 1 / sqrt(1 - beta2^t).  key seeds the stochastic
+ * rounding of 8-bit states.  Non-finite gradients make their parameter, and
+ * with 8-bit states the moments of their 256 values, non-finite. */
+int hv_adamw_step(void* const* params, const void* const* grads, const int64_t* numel, int tensors, int dtype,
+                  void* exp_avg, void* exp_avg_sq, float* avg_scale, float* sq_scale, int state_bits, float beta1,
+                  float one_minus_beta1, float beta2, float one_minus_beta2, float eps, float decay, float step_size,
+                  float inv_root_correction2, uint32_t key, void* stream);
+
+/* The fp32 values that 8-bit states stand for; second: 0 for exp_avg, 1 for
+ * exp_avg_sq.  count: a multiple of 256. */
+int hv_adamw_state_values(const uint8_t* codes, const float* scale, int64_t count, int second, float* out, void* stream);
+
+/* Self-attention over padded tokens with a learned (dq, dr, dz) offset bias
+ * per head (RelativeSelfAttention, fnn_transformer_net.py).
+ *   q [batch, queries, heads, head_dim]: the first `queries` tokens;
+ *   k, v [batch, tokens, heads, head_dim]; strides (batch, token, head) in
+ *   elements, the head's values contiguous;
+ *   token_q / token_r / token_z [batch, tokens] int32 and token_mask uint8
+ *   (0: masked), with their batch strides in token_stride (0: shared);
+ *   coordinates are clamped to +-2^19;
+ *   dq_bias, dr_bias [2 coord_clip + 1, heads], dz_bias [2 height_clip + 1, heads]
+ *   in table_dtype (fp32, or dtype).
+ * A masked token neither attends nor is attended to: its output row and its
+ * gradients are zero, and what its q, k and v hold is never used. */
+#define HV_ATTN_MAX_HEAD_DIM 64
+#define HV_ATTN_MAX_CLIP 16
+#define HV_ATTN_MAX_HEIGHT_CLIP 4
+
+typedef struct hv_attention {
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];
+    const int32_t *token_q, *token_r, *token_z;
+    const uint8_t* token_mask;
+    int64_t token_stride[4]; /* batch strides of token_q, token_r, token_z, token_mask */
+    const void *dq_bias, *dr_bias, *dz_bias;
+    int64_t batch;
+    int32_t tokens, queries, heads, head_dim, coord_clip, height_clip, dtype, table_dtype;
+    float scale;
+} hv_attention;
+
+/* saved: what the forward pass keeps for the backward pass (NULL where none
+ * follows; may be 0 bytes).  Workspaces: 256-byte aligned. */
+int hv_relative_attention_sizes(const hv_attention* a, size_t* saved_bytes, size_t* forward_bytes,
+                                size_t* backward_bytes);
+
+/* out: [batch, queries, heads, head_dim] contiguous. */
+int hv_relative_attention_forward(const hv_attention* a, void* out, void* saved, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* dout, dq: [batch, queries, heads, head_dim]; dk, dv share dkv_stride
+ * (strides: batch, token, head; the head's values contiguous).  The bias
+ * gradients are written in table_dtype.  Everything is overwritten. */
+int hv_relative_attention_backward(const hv_attention* a, const void* dout, const int64_t* dout_stride,
+                                   const void* saved, void* dq, void* dk, void* dv, const int64_t* dq_stride,
+                                   const int64_t* dkv_stride, void* ddq_bias, void* ddr_bias, void* ddz_bias, void* workspace,
+                                   size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
