@@ -27,7 +27,7 @@ struct AttnArgs {
     int64_t tqs, trs, tzs, ms;
     const uint8_t* mask;
     const void *bq, *br, *bz;
-    float *dbq, *dbr, *dbz;
+    void *dbq, *dbr, *dbz;
     float* p;   // workspace [B, H, Nq, N]
     float* ds;  // workspace [B, H, Nq, N]
     float* partial;

@@ -1,0 +1,221 @@
+// hv_mma.cuh -- warp matrix products of the attention kernels: m16n8 tiles of
+// mma.sync with fp32 accumulators, operands fp16, bf16, or fp32.
+//
+// The score tiles here are 16 x 8 pieces of at most a few dozen tokens with 8
+// to 64 values a head, and every one goes through the bias lookup and the
+// exponential in registers; a tcgen05 tile (128 rows, its accumulator in
+// tensor memory) would be mostly padding.
+//
+// fp32 operands are split in two tf32 halves, x = hi + lo, and a product is
+// hi hi + hi lo + lo hi: the dropped lo lo is below 2^-22 of it.
+//
+// Layouts (g = lane / 4, t = lane % 4).  C: c[0..1] row g, c[2..3] row g + 8,
+// columns 2t, 2t + 1.  The order of k inside a step is free as long as both
+// operands share it; fp32 steps (8 wide) pair k = t, t + 4 with columns 2t,
+// 2t + 1, so a C tile is an A operand without moving a value.
+#pragma once
+
+#include "hv_elem.cuh"
+
+namespace hv {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_addr(p)) : "memory");
+}
+__device__ __forceinline__ void ldsm2(uint32_t& a, uint32_t& b, const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(a), "=r"(b) : "r"(smem_addr(p)) : "memory");
+}
+__device__ __forceinline__ void ldsm2_t(uint32_t& a, uint32_t& b, const void* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                 : "=r"(a), "=r"(b) : "r"(smem_addr(p)) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+#define HV_MMA16(NAME, TYPE)                                                                                          \
+    __device__ __forceinline__ void NAME##_k16(float* c, const uint32_t* a, const uint32_t* b) {                      \
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                           \
+                     ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                                     \
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                 \
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));                             \
+    }                                                                                                                 \
+    __device__ __forceinline__ void NAME##_k8(float* c, const uint32_t* a, const uint32_t* b) {                       \
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32." TYPE "." TYPE ".f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};" \
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                 \
+                     : "r"(a[0]), "r"(a[1]), "r"(b[0]));                                                              \
+    }
+HV_MMA16(mma_f16, "f16")
+HV_MMA16(mma_bf16, "bf16")
+#undef HV_MMA16
+
+__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, const uint32_t* b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// hi: the value rounded to the 11 significant bits of tf32, lo: the rest,
+// rounded likewise (cut off instead, the errors would all have one sign).
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
+}
+
+// Tile operations of an element type.  D8: the step along the head's values
+// is 8 wide (16-bit types with 8 values a head).
+template <typename T, bool D8 = false>
+struct Tile {  // 16-bit types
+    static constexpr int KK = 16;           // step along tokens
+    static constexpr int KD = D8 ? 8 : 16;  // step along the head's values
+    struct A { uint32_t r[4]; };
+    struct B { uint32_t r[2]; };
+
+    __device__ static void mma(float* c, const A& a, const B& b) {
+        if constexpr (sizeof(T) == 2 && __is_same(T, __half)) mma_f16_k16(c, a.r, b.r);
+        else mma_bf16_k16(c, a.r, b.r);
+    }
+    __device__ static void mma_d(float* c, const A& a, const B& b) {
+        if constexpr (!D8) mma(c, a, b);
+        else if constexpr (__is_same(T, __half)) mma_f16_k8(c, a.r, b.r);
+        else mma_bf16_k8(c, a.r, b.r);
+    }
+    // 16 rows x KD values at p (row-major, ld elements a row)
+    __device__ static void load_a(A& a, const T* p, int ld, int lane) {
+        if constexpr (D8) ldsm2(a.r[0], a.r[1], p + (lane & 15) * ld);
+        else ldsm4(a.r, p + (lane & 15) * ld + (lane >> 4) * 8);
+    }
+    // 32 rows x KD values at p as four B operands (n = row)
+    __device__ static void load_bn(B (&b)[4], const T* p, int ld, int lane) {
+        uint32_t r[4];
+        ldsm4(r, p + lane * ld);
+#pragma unroll
+        for (int n = 0; n < 4; n++) b[n].r[0] = r[n];
+        if constexpr (!D8) {
+            ldsm4(r, p + lane * ld + 8);
+#pragma unroll
+            for (int n = 0; n < 4; n++) b[n].r[1] = r[n];
+        }
+    }
+    // KK rows x 8 values at p as a B operand (k = row)
+    __device__ static void load_bk(B& b, const T* p, int ld, int lane) { ldsm2_t(b.r[0], b.r[1], p + (lane & 15) * ld); }
+    // C tiles of 16 rows x KK columns as an A operand (k = column)
+    __device__ static void a_from_c(A& a, const float (*c)[4]) {
+        a.r[0] = pack2(c[0][0], c[0][1], T());
+        a.r[1] = pack2(c[0][2], c[0][3], T());
+        a.r[2] = pack2(c[1][0], c[1][1], T());
+        a.r[3] = pack2(c[1][2], c[1][3], T());
+    }
+};
+
+template <bool D8>
+struct Tile<float, D8> {
+    static constexpr int KK = 8, KD = 8;
+    struct A { uint32_t hi[4], lo[4]; };
+    struct B { uint32_t hi[2], lo[2]; };
+
+    __device__ static void mma(float* c, const A& a, const B& b) {
+        mma_tf32(c, a.lo, b.hi);
+        mma_tf32(c, a.hi, b.lo);
+        mma_tf32(c, a.hi, b.hi);
+    }
+    __device__ static void mma_d(float* c, const A& a, const B& b) { mma(c, a, b); }
+    __device__ static void load_a(A& a, const float* p, int ld, int lane) {
+        const float* q = p + (lane >> 2) * ld + 2 * (lane & 3);
+        const float2 x = *reinterpret_cast<const float2*>(q), y = *reinterpret_cast<const float2*>(q + 8 * ld);
+        split_tf32(x.x, a.hi[0], a.lo[0]);
+        split_tf32(y.x, a.hi[1], a.lo[1]);
+        split_tf32(x.y, a.hi[2], a.lo[2]);
+        split_tf32(y.y, a.hi[3], a.lo[3]);
+    }
+    __device__ static void load_bn(B (&b)[4], const float* p, int ld, int lane) {
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const float2 x = *reinterpret_cast<const float2*>(p + (8 * n + (lane >> 2)) * ld + 2 * (lane & 3));
+            split_tf32(x.x, b[n].hi[0], b[n].lo[0]);
+            split_tf32(x.y, b[n].hi[1], b[n].lo[1]);
+        }
+    }
+    __device__ static void load_bk(B& b, const float* p, int ld, int lane) {
+        const float* q = p + 2 * (lane & 3) * ld + (lane >> 2);
+        split_tf32(q[0], b.hi[0], b.lo[0]);
+        split_tf32(q[ld], b.hi[1], b.lo[1]);
+    }
+    __device__ static void a_from_c(A& a, const float (*c)[4]) {
+        split_tf32(c[0][0], a.hi[0], a.lo[0]);
+        split_tf32(c[0][2], a.hi[1], a.lo[1]);
+        split_tf32(c[0][1], a.hi[2], a.lo[2]);
+        split_tf32(c[0][3], a.hi[3], a.lo[3]);
+    }
+};
+
+// The transpose of 16 x 32 C tiles (rows: queries, columns: keys) as A operands
+// [2][16 / KK] (m = key, k = query): in registers for 16-bit types, through
+// 16 x kTransposeLd floats of the warp's own for fp32.
+constexpr int kTransposeLd = 36;
+
+template <typename T, bool D8>
+__device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[2][16 / Tile<T, D8>::KK], const float (&c)[4][4],
+                                            float* scratch, int lane) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            a[m][0].r[0] = transpose8(pack2(c[2 * m][0], c[2 * m][1], T()));
+            a[m][0].r[1] = transpose8(pack2(c[2 * m + 1][0], c[2 * m + 1][1], T()));
+            a[m][0].r[2] = transpose8(pack2(c[2 * m][2], c[2 * m][3], T()));
+            a[m][0].r[3] = transpose8(pack2(c[2 * m + 1][2], c[2 * m + 1][3], T()));
+        }
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            *reinterpret_cast<float2*>(scratch + g * kTransposeLd + 8 * n + 2 * t) = make_float2(c[n][0], c[n][1]);
+            *reinterpret_cast<float2*>(scratch + (g + 8) * kTransposeLd + 8 * n + 2 * t) = make_float2(c[n][2], c[n][3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float* p = scratch + (8 * k + 2 * t) * kTransposeLd + 16 * m + g;
+                split_tf32(p[0], a[m][k].hi[0], a[m][k].lo[0]);
+                split_tf32(p[8], a[m][k].hi[1], a[m][k].lo[1]);
+                split_tf32(p[kTransposeLd], a[m][k].hi[2], a[m][k].lo[2]);
+                split_tf32(p[kTransposeLd + 8], a[m][k].hi[3], a[m][k].lo[3]);
+            }
+    }
+}
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace hv

@@ -9,6 +9,7 @@
 
 #include "hv_adamw.cuh"
 #include "hv_attn.cuh"
+#include "hv_attn_short.cuh"
 #include "hv_norm.cuh"
 #include "../../include/hive_b200.h"
 
@@ -20,13 +21,16 @@ static inline int launched() { return cudaGetLastError() == cudaSuccess ? HV_OK 
 
 static inline size_t elem_bytes(int dtype) { return dtype == HV_F32 ? 4 : 2; }
 
+// SMs of the current device; 148 where there is none, so that workspace sizes
+// can be asked for without a device (a launch then fails by itself).
 static int sm_count() {
     static int n[64];
     static std::mutex mu;
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaGetLastError(), 148;
     std::lock_guard<std::mutex> lock(mu);
-    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) n[dev] = 0;
+    if (!n[dev] && cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        return cudaGetLastError(), 148;
     return n[dev];
 }
 
@@ -131,13 +135,113 @@ static int attn_shares(const hv_attention* a) {
     return (int)(rows < kHistShares ? (rows < 1 ? 1 : rows) : kHistShares);
 }
 
+// ---- up to 32 tokens
+constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kShortSmem = 100 * 1024;
+
+static bool attn_short(const hv_attention* a) { return a->tokens <= kSlots; }
+
+static int pad_dim(int D) { return D <= 8 ? 8 : D <= 16 ? 16 : D <= 32 ? 32 : 64; }
+
+// Heads a block: up to 8 (a warp each), fewer where their rows would leave an
+// SM with less than two blocks.
+static ShortPlan short_plan(const hv_attention* a, bool back) {
+    const int e = (int)elem_bytes(a->dtype), DP = pad_dim(a->head_dim), classes = attn_classes(a);
+    ShortPlan p = {};
+    for (p.groups = (a->heads + 7) / 8;; p.groups++) {
+        p.HG = (a->heads + p.groups - 1) / p.groups;
+        const int unit = e == 4 ? 32 : 16;  // rows an odd number of these apart do not meet in a bank
+        p.row = p.HG * DP * e;
+        if (p.row / unit % 2 == 0) p.row += unit;
+        p.stage = 3 * kSlots * 4 + (back ? 4 : 3) * kSlots * p.row;
+        const int floats = p.HG * classes * (back ? 33 : 1) + (back && e == 4 ? p.HG * 16 * kTransposeLd : 0);
+        p.tables = (int)((floats * 4 + 127) & ~127);
+        p.total = p.tables + 2 * p.stage;
+        if (p.total <= kShortSmem || p.HG == 1) break;
+    }
+    p.groups = (a->heads + p.HG - 1) / p.HG;
+    return p;
+}
+
+static bool strides_vec(const int64_t* s, int e) { return s[0] * e % 16 == 0 && s[1] * e % 16 == 0 && s[2] * e % 16 == 0; }
+
+static int short_blocks(const ShortPlan& p, int64_t batch, int resident) {
+    const int64_t n = ((int64_t)sm_count() * resident + p.groups - 1) / p.groups;
+    return (int)(batch < 1 ? 1 : batch < n ? batch : n);
+}
+
+static int short_resident(const ShortPlan& p) {  // at most, on an SM
+    const int by_smem = kSmemPerSm / (p.total + 1024), by_threads = 64 / p.HG;
+    return by_smem < by_threads ? (by_smem < 32 ? by_smem : 32) : (by_threads < 32 ? by_threads : 32);
+}
+
+// Shared-memory limit and resident blocks of a kernel, asked for once per
+// device and shape.
+template <typename K>
+static int resident_blocks(K kernel, int threads, int smem, int* out) {
+    struct Known { int threads, smem, blocks; };
+    static Known known[64];
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HV_ECUDA;
+    std::lock_guard<std::mutex> lock(mu);
+    Known& k = known[dev];
+    if (!k.blocks || k.threads != threads || k.smem != smem) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock) != cudaSuccess)
+            return HV_ECUDA;
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return HV_ECUDA;
+        k = {threads, smem, n};
+    }
+    *out = k.blocks;
+    return HV_OK;
+}
+
+template <typename T, bool BACK>
+static int launch_short(const AttnArgs& x, ShortPlan p, cudaStream_t st) {
+    auto go = [&](auto kernel) -> int {
+        int n = 0;
+        const int rc = resident_blocks(kernel, p.HG * 32, p.total, &n);
+        if (rc) return rc;
+        p.per_group = short_blocks(p, x.B, n < short_resident(p) ? n : short_resident(p));
+        kernel<<<p.per_group * p.groups, p.HG * 32, p.total, st>>>(x, p);
+        const int rc2 = launched();
+        if (rc2 || !BACK) return rc2;
+        const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
+        k_attn_table_sum<T><<<(classes * x.H + 3) / 4, 128, 0, st>>>(x.partial, p.per_group, W, classes, x.H, x.dbq, x.dbr,
+                                                                    x.dbz, x.t_f32);
+        return launched();
+    };
+    switch (pad_dim(x.D)) {
+        case 8: return go(k_attn_short<T, 8, BACK>);
+        case 16: return go(k_attn_short<T, 16, BACK>);
+        case 32: return go(k_attn_short<T, 32, BACK>);
+        default: return go(k_attn_short<T, 64, BACK>);
+    }
+}
+
+// 16-byte copies: whole pieces of every head, on 16-byte boundaries.
+static void short_vec(const AttnArgs& x, int e, bool back, ShortPlan* p) {
+    const bool d = x.D * e % 16 == 0;
+    p->vec_in = d && aligned(x.q, 16) && aligned(x.k, 16) && aligned(x.v, 16) && strides_vec(x.qs, e) && strides_vec(x.ks, e) &&
+                strides_vec(x.vs, e) && (!back || (aligned(x.dout, 16) && strides_vec(x.os, e)));
+    p->vec_out = d && strides_vec(x.gs, e) &&
+                 (back ? aligned(x.dq, 16) && aligned(x.dk, 16) && aligned(x.dv, 16) && strides_vec(x.gks, e) : aligned(x.out, 16));
+}
+
 struct AttnWorkspace {
     float *p, *ds, *partial;
     size_t bytes;
 };
 
 static AttnWorkspace attn_workspace(const hv_attention* a, bool back, void* base) {
-    AttnWorkspace w;
+    AttnWorkspace w = {};
+    if (attn_short(a)) {
+        if (!back) return w;
+        const ShortPlan p = short_plan(a, true);
+        w.partial = static_cast<float*>(base);
+        w.bytes = (size_t)short_blocks(p, a->batch, short_resident(p)) * attn_classes(a) * a->heads * 4;
+        return w;
+    }
     const size_t pairs = round256((size_t)a->batch * a->heads * a->queries * a->tokens * 4);
     char* c = static_cast<char*>(base);
     w.p = reinterpret_cast<float*>(c);
@@ -179,7 +283,6 @@ int hv_layer_norm_forward(const void* x, const void* residual, const void* weigh
     a.x = x, a.r = residual, a.w = weight, a.b = bias, a.s = sum, a.y = y, a.mean = mean, a.rstd = rstd;
     a.rows = rows, a.C = width, a.G = s.G, a.w_f32 = weight_dtype == HV_F32, a.eps = eps;
     const int grid = norm_grid(s, rows);
-    if (!grid) return HV_ECUDA;
     return by_type(dtype, [&](auto t) { return launch_norm<decltype(t), false>(a, s, grid, (cudaStream_t)stream); });
 }
 
@@ -187,8 +290,7 @@ int hv_layer_norm_workspace_bytes(int64_t rows, int width, int dtype, size_t* by
     NormShape s, t;
     if (!bytes || rows < 0 || width < 1 || width > kNormMaxWidth || dtype < 0 || dtype > 2) return HV_EINVAL;
     if (!norm_shape(width, dtype, false, &s) || !norm_shape(width, dtype, true, &t)) return HV_EINVAL;
-    const int64_t per = 148 * kNormBlocksPerSm;
-    *bytes = (size_t)(sm_count() ? (int64_t)sm_count() * kNormBlocksPerSm : per) * 2 * width * 4;
+    *bytes = (size_t)sm_count() * kNormBlocksPerSm * 2 * width * 4;
     return HV_OK;
 }
 
@@ -202,7 +304,6 @@ int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     NormShape s;
     if (!norm_shape(width, dtype, norm_vec(width, dtype, {dy, x, dsum, dx}), &s)) return HV_EINVAL;
     const int grid = rows ? norm_grid(s, rows) : 0;
-    if (rows && !grid) return HV_ECUDA;
     if (workspace_bytes < (size_t)grid * 2 * width * 4) return HV_EINVAL;
     NormArgs a = {};
     a.x = x, a.w = weight, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
@@ -301,9 +402,15 @@ int hv_relative_attention_forward(const hv_attention* a, void* out, void* saved,
     if (!attn_ok(a)) return HV_EINVAL;
     if (a->batch == 0 || a->queries == 0) return HV_OK;
     const AttnWorkspace w = attn_workspace(a, false, workspace);
-    if (!out || !workspace || !aligned(workspace, 256) || workspace_bytes < w.bytes) return HV_EINVAL;
+    if (!out || (w.bytes && (!workspace || !aligned(workspace, 256))) || workspace_bytes < w.bytes) return HV_EINVAL;
     AttnArgs x = attn_args(a);
     x.out = out, x.p = w.p;
+    x.gs[0] = (int64_t)x.Nq * x.H * x.D, x.gs[1] = (int64_t)x.H * x.D, x.gs[2] = x.D;
+    if (attn_short(a)) {
+        ShortPlan p = short_plan(a, false);
+        short_vec(x, (int)elem_bytes(a->dtype), false, &p);
+        return by_type(a->dtype, [&](auto t) { return launch_short<decltype(t), false>(x, p, (cudaStream_t)stream); });
+    }
     const int64_t grid = (x.B * x.H * x.Nq + 3) / 4;
     if (grid > 0x7fffffff) return HV_EINVAL;
     return by_type(a->dtype, [&](auto t) {
@@ -328,6 +435,12 @@ int hv_relative_attention_backward(const hv_attention* a, const void* dout, cons
     for (int i = 0; i < 3; i++) {
         x.os[i] = dout_stride ? dout_stride[i] : 0, x.gs[i] = dq_stride ? dq_stride[i] : 0;
         x.gks[i] = dkv_stride ? dkv_stride[i] : 0;
+    }
+    x.dbq = ddq_bias, x.dbr = ddr_bias, x.dbz = ddz_bias;
+    if (attn_short(a)) {
+        ShortPlan p = short_plan(a, true);
+        short_vec(x, (int)elem_bytes(a->dtype), true, &p);
+        return by_type(a->dtype, [&](auto t) { return launch_short<decltype(t), true>(x, p, (cudaStream_t)stream); });
     }
     const int64_t rows = (x.B * x.H * x.Nq + 3) / 4, keys = (x.B * x.H * x.N + 3) / 4;
     if (rows > 0x7fffffff || keys > 0x7fffffff) return HV_EINVAL;
