@@ -30,68 +30,67 @@ struct ShortPlan {
     int per_group;             // blocks for each group of heads
 };
 
-template <typename T>
-__device__ __forceinline__ T* row_ptr(void* base, const int64_t* s, int64_t b, int token, int head) {
-    return static_cast<T*>(base) + b * s[0] + token * s[1] + head * s[2];
-}
-
-// Rows of `n` tokens and the block's heads between global memory and the slots
-// of one operand; x: this thread's 16-byte piece of a row, r0 its first row.
+// The copies between global memory and the slots.  A unit is half the rows
+// (16) of one operand, and a warp's: 16-byte pieces, each lane at its own
+// place in a row, 32 / pieces rows at a time.
 template <typename T, int DP>
 struct RowCopy {
-    int heads, D, row, threads;
+    int D, row, width;
     bool vec;
-    int r0, rows, piece, head;  // vector copies
+    int r0, rows, at, lane, head, piece;  // 16-byte pieces: the lane's first row, rows at a time, its bytes in a slot
 
-    __device__ void init(int heads_, int D_, int row_, bool vec_) {
-        heads = heads_, D = D_, row = row_, vec = vec_, threads = blockDim.x;
-        const int per_head = D * (int)sizeof(T) / 16, chunks = heads * per_head;
+    __device__ void init(int heads, int D_, int row_, bool vec_) {
+        D = D_, row = row_, vec = vec_, width = heads * D_, lane = threadIdx.x & 31;
+        const int per_head = D * (int)sizeof(T) / 16, pieces = heads * per_head;
         if (vec) {
-            rows = threads / chunks, r0 = threadIdx.x / chunks;
-            const int x = threadIdx.x - r0 * chunks;
+            rows = 32 / pieces, r0 = lane / pieces;
+            const int x = lane - r0 * pieces;
             head = x / per_head, piece = x - head * per_head;
-            if (r0 >= rows) r0 = kSlots;  // threads past the last whole row
+            at = head * DP * (int)sizeof(T) + piece * 16;
+            if (r0 >= rows) r0 = kSlots;  // lanes past the last whole row
         }
     }
-    __device__ int at(int slot) const { return slot * row + head * DP * (int)sizeof(T) + piece * 16; }
+    __device__ static int slot(uint32_t valid, int r) { return __popc(valid & ((1u << r) - 1)); }
 
-    __device__ void load(char* dst, const void* src, const int64_t* s, int64_t b, int h0, int n, uint32_t valid) const {
-        const T* base = static_cast<const T*>(src) + b * s[0];
+    // half 0, 1: rows 16 half .. of the n tokens
+    __device__ void load(char* dst, const void* src, const int64_t* s, int64_t b, int h0, int n, int half,
+                         uint32_t valid) const {
+        const T* base = static_cast<const T*>(src) + b * s[0] + h0 * s[2];
+        const int end = min(n, 16 * half + 16);
         if (vec) {
-            const T* p = base + (h0 + head) * s[2] + piece * (16 / (int)sizeof(T));
-            for (int r = r0; r < n; r += rows)
-                if (valid >> r & 1) cp_async16(dst + at(__popc(valid & ((1u << r) - 1))), p + r * s[1]);
+            const T* p = base + head * s[2] + piece * (16 / (int)sizeof(T));
+            for (int r = 16 * half + r0; r < end; r += rows)
+                if (valid >> r & 1) cp_async16(dst + slot(valid, r) * row + at, p + r * s[1]);
         } else {
-            const int width = heads * D;
-            for (int i = threadIdx.x; i < n * width; i += threads) {
+            for (int i = 16 * half * width + lane; i < end * width; i += 32) {
                 const int r = i / width, c = i - r * width, h = c / D, d = c - h * D;
                 if (valid >> r & 1)
-                    reinterpret_cast<T*>(dst + __popc(valid & ((1u << r) - 1)) * row)[h * DP + d] =
-                        base[r * s[1] + (h0 + h) * s[2] + d];
+                    reinterpret_cast<T*>(dst + slot(valid, r) * row)[h * DP + d] = base[r * s[1] + h * s[2] + d];
             }
         }
-        // the slots up to the next multiple of 16 count as zero rows
-        const int c = __popc(valid & (n < 32 ? (1u << n) - 1 : 0xffffffffu)), end = (c + 15) & ~15;
-        for (int i = threadIdx.x; i < (end - c) * (row / 16); i += threads)
-            *reinterpret_cast<uint4*>(dst + c * row + i * 16) = make_uint4(0, 0, 0, 0);
+        if (half == 0) {  // the slots up to the next multiple of 16 count as zero rows
+            const int c = __popc(valid & (n < 32 ? (1u << n) - 1 : 0xffffffffu));
+            uint4* z = reinterpret_cast<uint4*>(dst + c * row);
+            for (int i = lane; i < (-c & 15) * (row >> 4); i += 32) z[i] = make_uint4(0, 0, 0, 0);
+        }
     }
-    __device__ void store(const char* src, void* dst, const int64_t* s, int64_t b, int h0, int n, uint32_t valid) const {
-        T* base = static_cast<T*>(dst) + b * s[0];
+    __device__ void store(const char* src, void* dst, const int64_t* s, int64_t b, int h0, int n, int half,
+                          uint32_t valid) const {
+        T* base = static_cast<T*>(dst) + b * s[0] + h0 * s[2];
+        const int end = min(n, 16 * half + 16);
         if (vec) {
-            T* p = base + (h0 + head) * s[2] + piece * (16 / (int)sizeof(T));
-            for (int r = r0; r < n; r += rows) {
+            T* p = base + head * s[2] + piece * (16 / (int)sizeof(T));
+            for (int r = 16 * half + r0; r < end; r += rows) {
                 uint4 v = make_uint4(0, 0, 0, 0);
-                if (valid >> r & 1) v = *reinterpret_cast<const uint4*>(src + at(__popc(valid & ((1u << r) - 1))));
+                if (valid >> r & 1) v = *reinterpret_cast<const uint4*>(src + slot(valid, r) * row + at);
                 *reinterpret_cast<uint4*>(p + r * s[1]) = v;
             }
         } else {
-            const int width = heads * D;
-            for (int i = threadIdx.x; i < n * width; i += threads) {
+            for (int i = 16 * half * width + lane; i < end * width; i += 32) {
                 const int r = i / width, c = i - r * width, h = c / D, d = c - h * D;
                 T v = from_f32<T>(0.f);
-                if (valid >> r & 1)
-                    v = reinterpret_cast<const T*>(src + __popc(valid & ((1u << r) - 1)) * row)[h * DP + d];
-                base[r * s[1] + (h0 + h) * s[2] + d] = v;
+                if (valid >> r & 1) v = reinterpret_cast<const T*>(src + slot(valid, r) * row)[h * DP + d];
+                base[r * s[1] + h * s[2] + d] = v;
             }
         }
     }
@@ -111,7 +110,7 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
     constexpr int NC = DP / 8;  // 8-value chunks of a head
     constexpr bool F32 = sizeof(T) == 4;
     extern __shared__ __align__(16) char smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
     const int group = blockIdx.x % p.groups, h0 = group * p.HG, heads = min(p.HG, a.H - h0);
     const int W = 2 * a.clip + 1, Z = 2 * a.clip_z + 1, classes = 2 * W + Z;
     const int ld = p.row / (int)sizeof(T);
@@ -169,10 +168,12 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                 for (int i = 0; i < 3; i++) c[i * kSlots] = coord(k.c[i]) * 4;
             }
             char* x = st + 3 * kSlots * 4;
-            in.load(x, a.q, a.qs, b, h0, a.Nq, valid);
-            in.load(x + operand, a.k, a.ks, b, h0, a.N, valid);
-            in.load(x + 2 * operand, a.v, a.vs, b, h0, a.N, valid);
-            if (BACK) in.load(x + 3 * operand, a.dout, a.os, b, h0, a.Nq, valid);
+            for (int u = warp; u < (BACK ? 8 : 6); u += warps) {
+                const int o = u >> 1;
+                const void* src = o == 0 ? a.q : o == 1 ? a.k : o == 2 ? a.v : a.dout;
+                const int64_t* s = o == 0 ? a.qs : o == 1 ? a.ks : o == 2 ? a.vs : a.os;
+                in.load(x + o * operand, src, s, b, h0, o == 0 || o == 3 ? a.Nq : a.N, u & 1, valid);
+            }
         }
         cp_async_commit();
         return valid;
@@ -243,11 +244,7 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (8 * i >= n) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) s[i][e] = -INFINITY;
-                        continue;
-                    }
+                    if (8 * i >= n) continue;
                     const int j = 8 * i + 2 * t;
                     const int2 kq = *reinterpret_cast<const int2*>(co + j), kr = *reinterpret_cast<const int2*>(co + kSlots + j),
                                kz = *reinterpret_cast<const int2*>(co + 2 * kSlots + j);
@@ -270,18 +267,20 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++) {
+                    if (8 * i >= n) continue;  // s stays 0 there
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         s[i][e] = exp2_approx(s[i][e] - top[e >> 1]);
                         sum[e >> 1] += s[i][e];
                     }
+                }
                 float delta[2] = {0.f, 0.f};
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                    sum[r] = 1.f / sum[r];
+                    sum[r] = rcp_approx(sum[r]);
                 }
                 if constexpr (!BACK) {
                     // o = p v; the division by the sum comes last
@@ -311,25 +310,25 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                     }
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                    for (int i = 0; i < 4; i++) {
+                        if (8 * i >= n) continue;
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             s[i][e] *= sum[e >> 1];
                             delta[e >> 1] = fmaf(s[i][e], dp[i][e], delta[e >> 1]);
                         }
+                    }
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 1);
                         delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 2);
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) dp[i][e] = s[i][e] * (dp[i][e] - delta[e >> 1]);
-                    // dp now holds ds
+                    // dp becomes ds; its sums by class
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if (8 * i >= n) continue;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) dp[i][e] = s[i][e] * (dp[i][e] - delta[e >> 1]);
                         const int j = 8 * i + 2 * t;
                         const int2 kq = *reinterpret_cast<const int2*>(co + j), kr = *reinterpret_cast<const int2*>(co + kSlots + j),
                                    kz = *reinterpret_cast<const int2*>(co + 2 * kSlots + j);
@@ -404,12 +403,10 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
             }
         }
         __syncthreads();
-        if (BACK) {
-            out.store(x, a.dq, a.gs, b, h0, a.Nq, valid);
-            out.store(x + operand, a.dk, a.gks, b, h0, a.N, valid);
-            out.store(x + 2 * operand, a.dv, a.gks, b, h0, a.N, valid);
-        } else {
-            out.store(x, a.out, a.gs, b, h0, a.Nq, valid);
+        for (int u = warp; u < (BACK ? 6 : 2); u += warps) {
+            const int o = u >> 1;
+            void* dst = !BACK ? a.out : o == 0 ? a.dq : o == 1 ? a.dk : a.dv;
+            out.store(x + o * operand, dst, o == 0 ? a.gs : a.gks, b, h0, o == 0 ? a.Nq : a.N, u & 1, valid);
         }
         __syncthreads();
         valid = valid_next;

@@ -143,7 +143,7 @@ static bool attn_short(const hv_attention* a) { return a->tokens <= kSlots; }
 static int pad_dim(int D) { return D <= 8 ? 8 : D <= 16 ? 16 : D <= 32 ? 32 : 64; }
 
 // Heads a block: up to 8 (a warp each), fewer where their rows would leave an
-// SM with less than two blocks.
+// SM with less than two blocks, or where a row is more than a warp's 512 bytes.
 static ShortPlan short_plan(const hv_attention* a, bool back) {
     const int e = (int)elem_bytes(a->dtype), DP = pad_dim(a->head_dim), classes = attn_classes(a);
     ShortPlan p = {};
@@ -156,7 +156,7 @@ static ShortPlan short_plan(const hv_attention* a, bool back) {
         const int floats = p.HG * classes * (back ? 33 : 1) + (back && e == 4 ? p.HG * 16 * kTransposeLd : 0);
         p.tables = (int)((floats * 4 + 127) & ~127);
         p.total = p.tables + 2 * p.stage;
-        if (p.total <= kShortSmem || p.HG == 1) break;
+        if ((p.total <= kShortSmem && p.HG * a->head_dim * e <= 512) || p.HG == 1) break;
     }
     p.groups = (a->heads + p.HG - 1) / p.HG;
     return p;
