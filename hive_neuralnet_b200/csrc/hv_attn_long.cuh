@@ -1,0 +1,588 @@
+// hv_attn_long.cuh -- the attention of hv_attn.cuh for any number of tokens:
+// one pass over the keys with the running maximum and sum of the softmax.
+//
+// A first kernel sorts each position's valid tokens to the front (order kept)
+// with their coordinates; everything after works on those slots, so a masked
+// token costs nothing but the zeros of its results.
+//
+// Forward and dq: a block takes 64 queries of one head, 16 a warp, and walks
+// over tiles of 64 keys, the next tile arriving while this one is computed.
+// With few queries a block takes 16 and its warps share each tile's keys; their
+// parts are joined at the end.  dk, dv: a block takes 64 keys, 16 a warp, and
+// walks over the queries with the scores transposed (rows: keys), so that the
+// probabilities are operands of both products as they stand.  The scores are
+// computed once more there: the sums over queries and over keys are both taken
+// in registers, in a fixed order, with no atomics.
+#pragma once
+
+#include "hv_attn.cuh"
+#include "hv_mma.cuh"
+
+namespace hv {
+
+constexpr int kTile = 64;          // tokens of a tile
+constexpr int kLongThreads = 128;
+constexpr float kLog2E = 1.4426950408889634f;
+
+struct LongArgs {
+    int4* meta;    // [B][Npad]: 4 x clamped coordinates, token
+    int2* count;   // [B]: valid tokens, valid queries
+    float* lse;    // [B][H][Qpad], log2 of the sum of exp2
+    float* o32;    // [B][H][Qpad][D], the output before rounding, by slot
+    float* delta;  // [B][H][Qpad]
+    int Npad, Qpad, tiles;  // tiles: query (key) tiles of a head
+    int vec_in;
+};
+
+// Row length of a tile in shared memory: an odd number of 16-byte (fp32: 32-byte) units.
+template <typename T, int DP>
+__host__ __device__ constexpr int tile_ld() {
+    return DP / 8 % 2 ? DP : DP + 8;
+}
+
+__global__ void __launch_bounds__(1024) k_attn_sort(const AttnArgs a, const LongArgs l) {
+    __shared__ int warp_sum[32], base[2];
+    const int64_t b = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint8_t* mask = a.mask + b * a.ms;
+    int4* meta = l.meta + b * l.Npad;
+    int valid = 0, queries = 0;
+    for (int j = threadIdx.x; j < a.N; j += blockDim.x) valid += mask[j] != 0, queries += mask[j] != 0 && j < a.Nq;
+    if (threadIdx.x == 0) base[0] = 0, base[1] = 0;
+    __syncthreads();
+    valid = __reduce_add_sync(0xffffffffu, valid), queries = __reduce_add_sync(0xffffffffu, queries);
+    if (lane == 0) atomicAdd(&base[0], valid), atomicAdd(&base[1], queries);
+    __syncthreads();
+    const int count = base[0];
+    if (threadIdx.x == 0) l.count[b] = make_int2(count, base[1]);
+    int before = 0;  // valid tokens before this chunk
+    for (int j0 = 0; j0 < a.N; j0 += blockDim.x) {
+        const int j = j0 + threadIdx.x;
+        const bool ok = j < a.N && mask[j];
+        const uint32_t m = __ballot_sync(0xffffffffu, ok);
+        __syncthreads();
+        if (lane == 0) warp_sum[warp] = __popc(m);
+        __syncthreads();
+        const int mine = __popc(m & ((1u << lane) - 1));
+        int prior = before;
+        for (int w = 0; w < (int)(blockDim.x >> 5); w++) {
+            if (w < warp) prior += warp_sum[w];
+            before += warp_sum[w];
+        }
+        if (j < a.N) {
+            const int slot = ok ? prior + mine : count + j - (prior + mine);
+            meta[slot] = make_int4(4 * coord(a.tq[b * a.tqs + j]), 4 * coord(a.tr[b * a.trs + j]),
+                                   4 * coord(a.tz[b * a.tzs + j]), j);
+        }
+    }
+    for (int j = a.N + threadIdx.x; j < l.Npad; j += blockDim.x) meta[j] = make_int4(0, 0, 0, 0);
+}
+
+// Rows of a tile, gathered by token.  Rows at or past `end` are zero.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void load_tile(T* dst, const T* src, int64_t stride, int D, const int4* meta, int end, bool vec) {
+    constexpr int LD = tile_ld<T, DP>(), E = 16 / sizeof(T);
+    if (vec) {
+        const int pieces = D / E, rows = kLongThreads / pieces, r0 = threadIdx.x / pieces, x = threadIdx.x - r0 * pieces;
+        if (r0 >= rows) return;
+        for (int r = r0; r < ROWS; r += rows) {
+            T* d = dst + r * LD + x * E;
+            if (r < end)
+                cp_async16(d, src + meta[r].w * stride + x * E);
+            else
+                *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        for (int i = threadIdx.x; i < ROWS * D; i += kLongThreads) {
+            const int r = i / D, d = i - r * D;
+            dst[r * LD + d] = r < end ? src[meta[r].w * stride + d] : from_f32<T>(0.f);
+        }
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias_table(float* tab, const AttnArgs& a, int h) {
+    const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
+    for (int c = threadIdx.x; c < classes; c += kLongThreads) {
+        const void* src = c < W ? a.bq : c < 2 * W ? a.br : a.bz;
+        tab[c] = kLog2E * load_param<T>(src, (int64_t)(c < W ? c : c < 2 * W ? c - W : c - 2 * W) * a.H + h, a.t_f32);
+    }
+}
+
+// The bias of a pair, and where its three classes are.
+struct BiasOf {
+    const char *q, *r, *z;
+    int top, top_z;
+    __device__ BiasOf(const float* tab, const AttnArgs& a) {
+        const int W = 2 * a.clip + 1;
+        q = reinterpret_cast<const char*>(tab), r = q + 4 * W, z = q + 8 * W, top = 8 * a.clip, top_z = 8 * a.clip_z;
+    }
+    __device__ __forceinline__ static float at(const char* p, int c) { return *reinterpret_cast<const float*>(p + c); }
+    // kq, kr, kz: the key's coordinates; qq, qr, qz: 4 clip less the query's
+    __device__ __forceinline__ void classes(int kq, int kr, int kz, int qq, int qr, int qz, int& cq, int& cr, int& cz) const {
+        cq = __viaddmin_s32_relu(kq, qq, top), cr = __viaddmin_s32_relu(kr, qr, top), cz = __viaddmin_s32_relu(kz, qz, top_z);
+    }
+    __device__ __forceinline__ float value(int cq, int cr, int cz) const { return at(q, cq) + at(r, cr) + at(z, cz); }
+};
+
+template <typename T, int DP>
+struct LongSmem {
+    static constexpr int LD = tile_ld<T, DP>();
+    static constexpr int kTileBytes = kTile * LD * (int)sizeof(T);
+    static constexpr int kMetaBytes = kTile * 16;
+};
+
+// BACK false: the forward pass; true: dq (and delta).  ROWS: 64, or 16 with
+// the keys of each tile shared by the warps.
+template <typename T, int DP, int ROWS, bool BACK>
+__global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, const LongArgs l) {
+    using Op = Tile<T, DP == 8>;
+    using S = LongSmem<T, DP>;
+    constexpr int LD = S::LD, NC = DP / 8;
+    constexpr bool SHARED = ROWS == 16;
+    constexpr int NT = SHARED ? 2 : 8;  // 8-key tiles of a warp
+    // The output before rounding gives the backward pass sum_j p dp, which it
+    // takes from every dp: 16-bit probabilities go into it in two parts.  The
+    // score gradients of the backward pass are rounded to the operands' type,
+    // like the results that they are summed into.
+    constexpr bool EXACT = !BACK && sizeof(T) == 2;
+    extern __shared__ __align__(16) char smem[];
+    T* sq = reinterpret_cast<T*>(smem);
+    T* sg = sq + ROWS * LD;
+    T* sk = sg + (BACK ? ROWS * LD : 0);  // two stages of k, then of v
+    T* sv = sk + 2 * kTile * LD;
+    int4* sm = reinterpret_cast<int4*>(sv + 2 * kTile * LD);  // three tiles of key meta
+    int4* qm = sm + 3 * kTile;                                // the queries' meta
+    float* tab = reinterpret_cast<float*>(qm + ROWS);
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
+    const int64_t b = blockIdx.x / l.tiles / a.H;
+    const int2 count = l.count[b];
+    const int q0 = tile * ROWS, n = count.x, nq = count.y - q0;  // nq: this tile's valid queries, if below ROWS
+    const int4* meta = l.meta + b * l.Npad;
+    const int64_t head = b * a.H + h;
+    T* out = BACK ? static_cast<T*>(a.dq) + b * a.gs[0] + h * a.gs[2] : static_cast<T*>(a.out) + b * a.gs[0] + h * a.gs[2];
+
+    // masked queries: zeros
+    for (int i = threadIdx.x; i < ROWS * a.D; i += kLongThreads) {
+        const int r = i / a.D, d = i - r * a.D;
+        if (r >= nq && q0 + r < a.Nq) out[meta[n + q0 + r - count.y].w * a.gs[1] + d] = from_f32<T>(0.f);
+    }
+    if (nq <= 0) return;
+
+    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2];
+    const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2];
+    const T* go = BACK ? static_cast<const T*>(a.dout) + b * a.os[0] + h * a.os[2] : nullptr;
+    if (a.D < DP) {  // the columns past D stay zero
+        uint4* z = reinterpret_cast<uint4*>(smem);
+        for (int i = threadIdx.x; i < (int)(reinterpret_cast<char*>(sm) - smem) / 16; i += kLongThreads) z[i] = make_uint4(0, 0, 0, 0);
+    }
+    load_bias_table<T>(tab, a, h);
+    for (int i = threadIdx.x; i < ROWS; i += kLongThreads) qm[i] = meta[min(q0 + i, l.Npad - 1)];
+    for (int i = threadIdx.x; i < kTile; i += kLongThreads) sm[i] = meta[i];
+    __syncthreads();
+    load_tile<T, DP, ROWS>(sq, q, a.qs[1], a.D, qm, nq, l.vec_in);
+    if (BACK) load_tile<T, DP, ROWS>(sg, go, a.os[1], a.D, qm, nq, l.vec_in);
+    const int tiles = (n + kTile - 1) / kTile;
+    auto issue = [&](int i) {  // keys of tile i, meta of tile i + 1
+        if (i < tiles) {
+            const int4* m = sm + i % 3 * kTile;
+            load_tile<T, DP, kTile>(sk + (i & 1) * kTile * LD, k, a.ks[1], a.D, m, n - i * kTile, l.vec_in);
+            load_tile<T, DP, kTile>(sv + (i & 1) * kTile * LD, v, a.vs[1], a.D, m, n - i * kTile, l.vec_in);
+            if (i + 1 < tiles && threadIdx.x < kTile)
+                cp_async16(sm + (i + 1) % 3 * kTile + threadIdx.x, meta + (i + 1) * kTile + threadIdx.x);
+        }
+        cp_async_commit();
+    };
+    issue(0);
+
+    const int row0 = SHARED ? 0 : warp * 16, key0 = SHARED ? warp * 16 : 0;
+    const BiasOf bias(tab, a);
+    const float scale2 = a.scale * kLog2E;
+    int qq[2], qr[2], qz[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int4 m = qm[row0 + g + 8 * r];
+        qq[r] = 4 * a.clip - m.x, qr[r] = 4 * a.clip - m.y, qz[r] = 4 * a.clip_z - m.z;
+    }
+    float lse[2] = {0.f, 0.f}, delta[2] = {0.f, 0.f};
+    if (BACK) {
+        // delta = sum over the head of dout times the output before rounding: four lanes a row
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = row0 + g + 8 * r;
+            if (row < nq) {
+                const int64_t at = head * l.Qpad + q0 + row;
+                lse[r] = l.lse[at];
+                const float* o = l.o32 + at * a.D;
+                const T* d = go + qm[row].w * a.os[1];
+                for (int c = t; c < a.D; c += 4) delta[r] = fmaf(o[c], to_f32(d[c]), delta[r]);
+            }
+            delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 1);
+            delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 2);
+            if (row < nq && t == 0 && (!SHARED || warp == 0)) l.delta[head * l.Qpad + q0 + row] = delta[r];
+        }
+    }
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[NC][4];
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[c][e] = 0.f;
+
+    for (int i = 0; i < tiles; i++) {
+        cp_async_wait<0>();
+        __syncthreads();
+        issue(i + 1);
+        const T* tk = sk + (i & 1) * kTile * LD + key0 * LD;
+        const T* tv = sv + (i & 1) * kTile * LD + key0 * LD;
+        const int4* tm = sm + i % 3 * kTile + key0;
+        const int left = n - i * kTile - key0;  // valid keys of this warp's part
+        float s[NT][4], dp[BACK ? NT : 1][4];
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[j][e] = 0.f;
+                if (BACK) dp[j][e] = 0.f;
+            }
+        constexpr int NB = SHARED ? 2 : 4;
+#pragma unroll
+        for (int d = 0; d < DP; d += Op::KD) {
+            typename Op::A qa;
+            Op::load_a(qa, sq + row0 * LD + d, LD, lane);
+#pragma unroll
+            for (int j = 0; j < NT; j += NB) {
+                typename Op::B kb[NB];
+                Op::load_bn(kb, tk + j * 8 * LD + d, LD, lane);
+#pragma unroll
+                for (int x = 0; x < NB; x++) Op::mma_d(s[j + x], qa, kb[x]);
+            }
+            if constexpr (BACK) {
+                Op::load_a(qa, sg + row0 * LD + d, LD, lane);
+#pragma unroll
+                for (int j = 0; j < NT; j += NB) {
+                    typename Op::B vb[NB];
+                    Op::load_bn(vb, tv + j * 8 * LD + d, LD, lane);
+#pragma unroll
+                    for (int x = 0; x < NB; x++) Op::mma_d(dp[j + x], qa, vb[x]);
+                }
+            }
+        }
+        float high[2] = {top[0], top[1]};
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int r = e >> 1;
+                int cq, cr, cz;
+                bias.classes(e & 1 ? mb.x : ma.x, e & 1 ? mb.y : ma.y, e & 1 ? mb.z : ma.z, qq[r], qr[r], qz[r], cq, cr, cz);
+                s[j][e] = fmaf(s[j][e], scale2, bias.value(cq, cr, cz));
+                if (8 * j + 2 * t + (e & 1) >= left) s[j][e] = -INFINITY;
+                if (!BACK) high[r] = fmaxf(high[r], s[j][e]);
+            }
+        }
+        if constexpr (!BACK) {
+            float base[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], 1));
+                high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], 2));
+                base[r] = high[r] == -INFINITY ? 0.f : high[r];  // no key of this warp's yet
+                const float f = exp2_approx(top[r] - base[r]);
+                top[r] = high[r];
+                sum[r] *= f;
+#pragma unroll
+                for (int c = 0; c < NC; c++) acc[c][2 * r] *= f, acc[c][2 * r + 1] *= f;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[j][e] = exp2_approx(s[j][e] - base[e >> 1]);
+                    sum[e >> 1] += s[j][e];
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    s[j][e] = exp2_approx(s[j][e] - lse[e >> 1]) * (dp[j][e] - delta[e >> 1]);
+        }
+        const T* tb = BACK ? tk : tv;
+#pragma unroll
+        for (int x = 0; x < NT * 8; x += Op::KK) {
+            typename Op::A pa, pb;
+            Op::a_from_c(pa, s + x / 8);
+            if constexpr (EXACT) Op::a_rest(pb, pa, s + x / 8);
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                typename Op::B vb;
+                Op::load_bk(vb, tb + x * LD + 8 * c, LD, lane);
+                Op::mma(acc[c], pa, vb);
+                if constexpr (EXACT) Op::mma(acc[c], pb, vb);
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    }
+    float inv[2] = {a.scale, a.scale};
+    if (SHARED) {
+        // join the warps' parts, in their order, in warp 0
+        __syncthreads();
+        float* join = reinterpret_cast<float*>(smem);  // [warp][16 rows][DP + 2]
+        constexpr int JL = DP + 2;
+        float* mine = join + warp * 16 * JL;
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) mine[(g + 8 * r) * JL + 8 * c + 2 * t + e] = acc[c][2 * r + e];
+            if (t == 0) mine[(g + 8 * r) * JL + DP] = top[r], mine[(g + 8 * r) * JL + DP + 1] = sum[r];
+        }
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const float* p = join + (g + 8 * r) * JL;
+            float high = -INFINITY, w[4];
+            for (int x = 0; x < 4; x++) high = fmaxf(high, p[x * 16 * JL + DP]);
+            sum[r] = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                w[x] = BACK ? 1.f : exp2_approx(p[x * 16 * JL + DP] - high);
+                sum[r] += w[x] * p[x * 16 * JL + DP + 1];
+            }
+            top[r] = high;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float z = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) z = fmaf(w[x], p[x * 16 * JL + 8 * c + 2 * t + e], z);
+                    acc[c][2 * r + e] = z;
+                }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int row = row0 + g + 8 * r;
+        if (row >= nq) continue;
+        const int64_t at = head * l.Qpad + q0 + row;
+        if (!BACK) {
+            inv[r] = 1.f / sum[r];
+            if (l.lse && t == 0) l.lse[at] = top[r] + log2f(sum[r]);
+        }
+        T* dst = out + qm[row].w * a.gs[1];
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = 8 * c + 2 * t + e;
+                if (d >= a.D) continue;
+                const float o = acc[c][2 * r + e] * inv[r];
+                dst[d] = from_f32<T>(o);
+                if (!BACK && l.o32) l.o32[at * a.D + d] = o;
+            }
+    }
+}
+
+// dk, dv and the bias sums of 64 keys of one head.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, const LongArgs l) {
+    using Op = Tile<T, DP == 8>;
+    using S = LongSmem<T, DP>;
+    constexpr int LD = S::LD, NC = DP / 8;
+    extern __shared__ __align__(16) char smem[];
+    T* sk = reinterpret_cast<T*>(smem);
+    T* sv = sk + kTile * LD;
+    T* sq = sv + kTile * LD;  // two stages of q, then of dout
+    T* sg = sq + 2 * kTile * LD;
+    int4* sm = reinterpret_cast<int4*>(sg + 2 * kTile * LD);  // three tiles of query meta
+    int4* km = sm + 3 * kTile;                                // the keys' meta
+    float2* sd = reinterpret_cast<float2*>(km + kTile);       // two tiles of (lse, delta)
+    float* tab = reinterpret_cast<float*>(sd + 2 * kTile);
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
+    const int64_t b = blockIdx.x / l.tiles / a.H;
+    const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
+    float* hist = tab + classes;
+    const int2 count = l.count[b];
+    const int k0 = tile * kTile, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below 64
+    const int4* meta = l.meta + b * l.Npad;
+    const int64_t head = b * a.H + h;
+    float* part = a.partial + ((b * l.tiles + tile) * classes) * a.H + h;
+    T* dk = static_cast<T*>(a.dk) + b * a.gks[0] + h * a.gks[2];
+    T* dv = static_cast<T*>(a.dv) + b * a.gks[0] + h * a.gks[2];
+    for (int i = threadIdx.x; i < kTile * a.D; i += kLongThreads) {  // masked keys: zeros
+        const int r = i / a.D, d = i - r * a.D;
+        if (r >= n && k0 + r < a.N) {
+            const int64_t at = meta[k0 + r].w * a.gks[1] + d;
+            dk[at] = dv[at] = from_f32<T>(0.f);
+        }
+    }
+    if (n <= 0) {
+        for (int c = threadIdx.x; c < classes; c += kLongThreads) part[(int64_t)c * a.H] = 0.f;
+        return;
+    }
+    const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
+    const T* go = static_cast<const T*>(a.dout) + b * a.os[0] + h * a.os[2];
+    if (a.D < DP) {
+        uint4* z = reinterpret_cast<uint4*>(smem);
+        for (int i = threadIdx.x; i < (int)(reinterpret_cast<char*>(sm) - smem) / 16; i += kLongThreads) z[i] = make_uint4(0, 0, 0, 0);
+    }
+    load_bias_table<T>(tab, a, h);
+    for (int i = threadIdx.x; i < classes * kLongThreads; i += kLongThreads) hist[i] = 0.f;
+    for (int i = threadIdx.x; i < kTile; i += kLongThreads) km[i] = meta[k0 + i], sm[i] = meta[i];
+    __syncthreads();
+    load_tile<T, DP, kTile>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, kTile>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
+    const int tiles = (nq + kTile - 1) / kTile;
+    auto issue = [&](int i) {
+        if (i < tiles) {
+            const int4* m = sm + i % 3 * kTile;
+            load_tile<T, DP, kTile>(sq + (i & 1) * kTile * LD, q, a.qs[1], a.D, m, nq - i * kTile, l.vec_in);
+            load_tile<T, DP, kTile>(sg + (i & 1) * kTile * LD, go, a.os[1], a.D, m, nq - i * kTile, l.vec_in);
+            if (threadIdx.x < kTile) {
+                const int s = i * kTile + threadIdx.x;
+                // past the last query: a probability of zero
+                float2 x = make_float2(INFINITY, 0.f);
+                if (s < nq) x = make_float2(l.lse[head * l.Qpad + s], l.delta[head * l.Qpad + s]);
+                sd[(i & 1) * kTile + threadIdx.x] = x;
+                if (i + 1 < tiles)
+                    cp_async16(sm + (i + 1) % 3 * kTile + threadIdx.x, meta + (i + 1) * kTile + threadIdx.x);
+            }
+        }
+        cp_async_commit();
+    };
+    issue(0);
+    const BiasOf bias(tab, a);
+    const float scale2 = a.scale * kLog2E;
+    char* sums = reinterpret_cast<char*>(hist + warp * classes * 32 + lane);
+    int kq[2], kr[2], kz[2];
+    bool live[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int4 m = km[warp * 16 + g + 8 * r];
+        kq[r] = m.x + 4 * a.clip, kr[r] = m.y + 4 * a.clip, kz[r] = m.z + 4 * a.clip_z;
+        live[r] = warp * 16 + g + 8 * r < n;
+    }
+    float ak[NC][4], av[NC][4];
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) ak[c][e] = av[c][e] = 0.f;
+
+    for (int i = 0; i < tiles; i++) {
+        cp_async_wait<0>();
+        __syncthreads();
+        issue(i + 1);
+#pragma unroll 1
+        for (int y = 0; y < kTile; y += 32) {  // 32 queries at a time
+            if (i * kTile + y >= nq) break;
+            const T* tq = sq + ((i & 1) * kTile + y) * LD;
+            const T* tg = sg + ((i & 1) * kTile + y) * LD;
+            const int4* tm = sm + i % 3 * kTile + y;
+            const float2* td = sd + (i & 1) * kTile + y;
+            float s[4][4], dp[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[j][e] = dp[j][e] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DP; d += Op::KD) {
+                typename Op::A ka;
+                typename Op::B qb[4];
+                Op::load_a(ka, sk + warp * 16 * LD + d, LD, lane);
+                Op::load_bn(qb, tq + d, LD, lane);
+#pragma unroll
+                for (int x = 0; x < 4; x++) Op::mma_d(s[x], ka, qb[x]);
+                Op::load_a(ka, sv + warp * 16 * LD + d, LD, lane);
+                Op::load_bn(qb, tg + d, LD, lane);
+#pragma unroll
+                for (int x = 0; x < 4; x++) Op::mma_d(dp[x], ka, qb[x]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
+                const float2 da = td[8 * j + 2 * t], db = td[8 * j + 2 * t + 1];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int r = e >> 1;
+                    int cq, cr, cz;
+                    bias.classes(kq[r], kr[r], kz[r], -(e & 1 ? mb.x : ma.x), -(e & 1 ? mb.y : ma.y), -(e & 1 ? mb.z : ma.z), cq,
+                                 cr, cz);
+                    const float x = fmaf(s[j][e], scale2, bias.value(cq, cr, cz));
+                    s[j][e] = live[r] ? exp2_approx(x - (e & 1 ? db.x : da.x)) : 0.f;
+                    dp[j][e] = s[j][e] * (dp[j][e] - (e & 1 ? db.y : da.y));
+                    float* hq = reinterpret_cast<float*>(sums + cq * 32);
+                    float* hr = reinterpret_cast<float*>(sums + W * 128 + cr * 32);
+                    float* hz = reinterpret_cast<float*>(sums + 2 * W * 128 + cz * 32);
+                    const float xq = *hq, xr = *hr, xz = *hz;
+                    *hq = xq + dp[j][e];
+                    *hr = xr + dp[j][e];
+                    *hz = xz + dp[j][e];
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 32; x += Op::KK) {
+                typename Op::A pa;
+                Op::a_from_c(pa, s + x / 8);
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    typename Op::B gb;
+                    Op::load_bk(gb, tg + x * LD + 8 * c, LD, lane);
+                    Op::mma(av[c], pa, gb);
+                }
+                Op::a_from_c(pa, dp + x / 8);
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    typename Op::B qb;
+                    Op::load_bk(qb, tq + x * LD + 8 * c, LD, lane);
+                    Op::mma(ak[c], pa, qb);
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        const int row = warp * 16 + g + 8 * r;
+        if (row >= n) continue;
+        const int64_t at = km[row].w * a.gks[1];
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = 8 * c + 2 * t + e;
+                if (d >= a.D) continue;
+                dk[at + d] = from_f32<T>(ak[c][2 * r + e] * a.scale);
+                dv[at + d] = from_f32<T>(av[c][2 * r + e]);
+            }
+    }
+    // this block's sums: a lane a class over its warp's 32 columns, then the warps
+    __syncthreads();
+    for (int c = lane; c < classes; c += 32) {
+        const float* col = hist + (warp * classes + c) * 32;
+        float x = 0.f;
+        for (int i = 0; i < 32; i++) x += col[(i + lane) & 31];
+        hist[(warp * classes + c) * 32] = x;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < classes; c += kLongThreads) {
+        float x = 0.f;
+        for (int w = 0; w < 4; w++) x += hist[(w * classes + c) * 32];
+        part[(int64_t)c * a.H] = x;
+    }
+}
+
+}  // namespace hv

@@ -51,6 +51,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ float2 unpack2(uint32_t x, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+__device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) {
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+
 #define HV_MMA16(NAME, TYPE)                                                                                          \
     __device__ __forceinline__ void NAME##_k16(float* c, const uint32_t* a, const uint32_t* b) {                      \
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                           \
@@ -103,7 +108,16 @@ struct Tile {  // 16-bit types
         if constexpr (D8) ldsm2(a.r[0], a.r[1], p + (lane & 15) * ld);
         else ldsm4(a.r, p + (lane & 15) * ld + (lane >> 4) * 8);
     }
-    // 32 rows x KD values at p as four B operands (n = row)
+    // 16 or 32 rows x KD values at p as B operands (n = row)
+    __device__ static void load_bn(B (&b)[2], const T* p, int ld, int lane) {
+        if constexpr (D8) {
+            ldsm2(b[0].r[0], b[1].r[0], p + (lane & 15) * ld);
+        } else {
+            uint32_t r[4];
+            ldsm4(r, p + (lane & 15) * ld + (lane >> 4) * 8);
+            b[0].r[0] = r[0], b[1].r[0] = r[1], b[0].r[1] = r[2], b[1].r[1] = r[3];
+        }
+    }
     __device__ static void load_bn(B (&b)[4], const T* p, int ld, int lane) {
         uint32_t r[4];
         ldsm4(r, p + lane * ld);
@@ -117,6 +131,15 @@ struct Tile {  // 16-bit types
     }
     // KK rows x 8 values at p as a B operand (k = row)
     __device__ static void load_bk(B& b, const T* p, int ld, int lane) { ldsm2_t(b.r[0], b.r[1], p + (lane & 15) * ld); }
+    // What a_from_c left of the C tiles, as a second operand: with it a product
+    // has 16 (fp16: 22) bits of them instead of 8 (11).
+    __device__ static void a_rest(A& a, const A& first, const float (*c)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = unpack2(first.r[i], T());
+            a.r[i] = pack2(c[i >> 1][2 * (i & 1)] - f.x, c[i >> 1][2 * (i & 1) + 1] - f.y, T());
+        }
+    }
     // C tiles of 16 rows x KK columns as an A operand (k = column)
     __device__ static void a_from_c(A& a, const float (*c)[4]) {
         a.r[0] = pack2(c[0][0], c[0][1], T());
@@ -146,9 +169,10 @@ struct Tile<float, D8> {
         split_tf32(x.y, a.hi[2], a.lo[2]);
         split_tf32(y.y, a.hi[3], a.lo[3]);
     }
-    __device__ static void load_bn(B (&b)[4], const float* p, int ld, int lane) {
+    template <int NB>
+    __device__ static void load_bn(B (&b)[NB], const float* p, int ld, int lane) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) {
+        for (int n = 0; n < NB; n++) {
             const float2 x = *reinterpret_cast<const float2*>(p + (8 * n + (lane >> 2)) * ld + 2 * (lane & 3));
             split_tf32(x.x, b[n].hi[0], b[n].lo[0]);
             split_tf32(x.y, b[n].hi[1], b[n].lo[1]);

@@ -9,6 +9,7 @@
 
 #include "hv_adamw.cuh"
 #include "hv_attn.cuh"
+#include "hv_attn_long.cuh"
 #include "hv_attn_short.cuh"
 #include "hv_norm.cuh"
 #include "../../include/hive_b200.h"
@@ -123,17 +124,12 @@ static bool attn_ok(const hv_attention* a) {
         a->height_clip > HV_ATTN_MAX_HEIGHT_CLIP)
         return false;
     if (a->heads > 65535) return false;
-    if (a->batch == 0 || a->queries == 0) return true;
-    return a->q && a->k && a->v && a->token_q && a->token_r && a->token_z && a->token_mask && a->dq_bias &&
+    if (a->batch == 0 || a->tokens == 0) return true;
+    return (a->q || a->queries == 0) && a->k && a->v && a->token_q && a->token_r && a->token_z && a->token_mask && a->dq_bias &&
            a->dr_bias && a->dz_bias;
 }
 
 static int attn_classes(const hv_attention* a) { return 2 * (2 * a->coord_clip + 1) + 2 * a->height_clip + 1; }
-
-static int attn_shares(const hv_attention* a) {
-    const int64_t rows = a->batch * a->queries;
-    return (int)(rows < kHistShares ? (rows < 1 ? 1 : rows) : kHistShares);
-}
 
 // ---- up to 32 tokens
 constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kShortSmem = 100 * 1024;
@@ -207,8 +203,8 @@ static int launch_short(const AttnArgs& x, ShortPlan p, cudaStream_t st) {
         const int rc2 = launched();
         if (rc2 || !BACK) return rc2;
         const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
-        k_attn_table_sum<T><<<(classes * x.H + 3) / 4, 128, 0, st>>>(x.partial, p.per_group, W, classes, x.H, x.dbq, x.dbr,
-                                                                    x.dbz, x.t_f32);
+        k_attn_table_sum<T><<<(classes * x.H + 7) / 8, 1024, 0, st>>>(x.partial, p.per_group, W, classes, x.H, x.dbq, x.dbr,
+                                                                     x.dbz, x.t_f32);
         return launched();
     };
     switch (pad_dim(x.D)) {
@@ -220,35 +216,106 @@ static int launch_short(const AttnArgs& x, ShortPlan p, cudaStream_t st) {
 }
 
 // 16-byte copies: whole pieces of every head, on 16-byte boundaries.
-static void short_vec(const AttnArgs& x, int e, bool back, ShortPlan* p) {
-    const bool d = x.D * e % 16 == 0;
-    p->vec_in = d && aligned(x.q, 16) && aligned(x.k, 16) && aligned(x.v, 16) && strides_vec(x.qs, e) && strides_vec(x.ks, e) &&
-                strides_vec(x.vs, e) && (!back || (aligned(x.dout, 16) && strides_vec(x.os, e)));
-    p->vec_out = d && strides_vec(x.gs, e) &&
-                 (back ? aligned(x.dq, 16) && aligned(x.dk, 16) && aligned(x.dv, 16) && strides_vec(x.gks, e) : aligned(x.out, 16));
+static bool vec_in(const AttnArgs& x, int e, bool back) {
+    return x.D * e % 16 == 0 && aligned(x.q, 16) && aligned(x.k, 16) && aligned(x.v, 16) && strides_vec(x.qs, e) &&
+           strides_vec(x.ks, e) && strides_vec(x.vs, e) && (!back || (aligned(x.dout, 16) && strides_vec(x.os, e)));
 }
 
-struct AttnWorkspace {
-    float *p, *ds, *partial;
-    size_t bytes;
-};
+static bool vec_out(const AttnArgs& x, int e, bool back) {
+    return x.D * e % 16 == 0 && strides_vec(x.gs, e) &&
+           (back ? aligned(x.dq, 16) && aligned(x.dk, 16) && aligned(x.dv, 16) && strides_vec(x.gks, e) : aligned(x.out, 16));
+}
 
-static AttnWorkspace attn_workspace(const hv_attention* a, bool back, void* base) {
-    AttnWorkspace w = {};
-    if (attn_short(a)) {
-        if (!back) return w;
-        const ShortPlan p = short_plan(a, true);
-        w.partial = static_cast<float*>(base);
-        w.bytes = (size_t)short_blocks(p, a->batch, short_resident(p)) * attn_classes(a) * a->heads * 4;
-        return w;
-    }
-    const size_t pairs = round256((size_t)a->batch * a->heads * a->queries * a->tokens * 4);
+// ---- any number of tokens
+static int round_up(int x, int n) { return (x + n - 1) / n * n; }
+
+// What the forward pass leaves for the backward pass (or, without one, its
+// workspace: the first two alone).
+static size_t long_saved(const hv_attention* a, void* base, bool all, LongArgs* l) {
+    l->Npad = round_up(a->tokens, kTile), l->Qpad = round_up(a->queries, kTile);
     char* c = static_cast<char*>(base);
-    w.p = reinterpret_cast<float*>(c);
-    w.ds = reinterpret_cast<float*>(c + pairs);
-    w.partial = reinterpret_cast<float*>(c + 2 * pairs);
-    w.bytes = back ? 2 * pairs + (size_t)attn_shares(a) * attn_classes(a) * a->heads * 4 : pairs;
-    return w;
+    size_t n = 0;
+    auto take = [&](size_t bytes) {
+        char* p = c ? c + n : nullptr;
+        n += round256(bytes);
+        return p;
+    };
+    const size_t rows = (size_t)a->batch * a->heads * l->Qpad;
+    l->meta = reinterpret_cast<int4*>(take((size_t)a->batch * l->Npad * sizeof(int4)));
+    l->count = reinterpret_cast<int2*>(take((size_t)a->batch * sizeof(int2)));
+    l->lse = nullptr, l->o32 = nullptr;
+    if (all) {
+        l->lse = reinterpret_cast<float*>(take(rows * 4));
+        l->o32 = reinterpret_cast<float*>(take(rows * a->head_dim * 4));
+    }
+    return n;
+}
+
+static size_t long_workspace(const hv_attention* a, void* base, LongArgs* l, float** partial) {
+    const size_t delta = round256((size_t)a->batch * a->heads * round_up(a->queries, kTile) * 4);
+    const int64_t blocks = a->batch * (round_up(a->tokens, kTile) / kTile);
+    l->delta = static_cast<float*>(base);
+    *partial = base ? reinterpret_cast<float*>(static_cast<char*>(base) + delta) : nullptr;
+    return delta + (size_t)blocks * attn_classes(a) * a->heads * 4;
+}
+
+// 16 queries a block where blocks of 64 would leave SMs without one.
+static bool few_queries(const AttnArgs& x) {
+    return x.Nq <= 16 || x.B * x.H * ((x.Nq + kTile - 1) / kTile) < sm_count();
+}
+
+template <typename T, int DP, int ROWS, bool BACK>
+static int launch_query(const AttnArgs& x, LongArgs l, cudaStream_t st) {
+    constexpr int LD = tile_ld<T, DP>();
+    const int classes = 2 * (2 * x.clip + 1) + 2 * x.clip_z + 1;
+    const int smem = (ROWS * (BACK ? 2 : 1) + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + ROWS) * 16 + classes * 4;
+    l.tiles = (x.Nq + ROWS - 1) / ROWS;
+    const int64_t grid = x.B * x.H * l.tiles;
+    if (grid > 0x7fffffff) return HV_EINVAL;
+    int n = 0;
+    const int rc = resident_blocks(k_attn_query<T, DP, ROWS, BACK>, kLongThreads, smem, &n);
+    if (rc) return rc;
+    k_attn_query<T, DP, ROWS, BACK><<<(unsigned)grid, kLongThreads, smem, st>>>(x, l);
+    return launched();
+}
+
+template <typename T, int DP>
+static int launch_keys(const AttnArgs& x, LongArgs l, cudaStream_t st) {
+    constexpr int LD = tile_ld<T, DP>();
+    const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
+    const int smem = 6 * kTile * LD * (int)sizeof(T) + 4 * kTile * 16 + 2 * kTile * 8 + classes * 4 * (1 + kLongThreads);
+    l.tiles = (x.N + kTile - 1) / kTile;
+    const int64_t grid = x.B * x.H * l.tiles;
+    if (grid > 0x7fffffff) return HV_EINVAL;
+    int n = 0;
+    int rc = resident_blocks(k_attn_keys<T, DP>, kLongThreads, smem, &n);
+    if (rc) return rc;
+    if (grid) {
+        k_attn_keys<T, DP><<<(unsigned)grid, kLongThreads, smem, st>>>(x, l);
+        if ((rc = launched())) return rc;
+    }
+    k_attn_table_sum<T><<<(classes * x.H + 7) / 8, 1024, 0, st>>>(x.partial, x.B * l.tiles, W, classes, x.H, x.dbq, x.dbr, x.dbz,
+                                                                 x.t_f32);
+    return launched();
+}
+
+template <typename T, bool BACK>
+static int launch_long(const AttnArgs& x, const LongArgs& l, cudaStream_t st) {
+    auto go = [&](auto dim) -> int {
+        constexpr int DP = decltype(dim)::value;
+        int rc = HV_OK;
+        if (x.B && x.Nq)
+            rc = few_queries(x) ? launch_query<T, DP, 16, BACK>(x, l, st) : launch_query<T, DP, 64, BACK>(x, l, st);
+        if constexpr (BACK)
+            if (!rc) rc = launch_keys<T, DP>(x, l, st);
+        return rc;
+    };
+    switch (pad_dim(x.D)) {
+        case 8: return go(std::integral_constant<int, 8>());
+        case 16: return go(std::integral_constant<int, 16>());
+        case 32: return go(std::integral_constant<int, 32>());
+        default: return go(std::integral_constant<int, 64>());
+    }
 }
 
 static AttnArgs attn_args(const hv_attention* a) {
@@ -390,79 +457,81 @@ int hv_adamw_state_values(const uint8_t* codes, const float* scale, int64_t coun
 
 int hv_relative_attention_sizes(const hv_attention* a, size_t* saved_bytes, size_t* forward_bytes, size_t* backward_bytes) {
     if (!attn_ok(a) || !saved_bytes || !forward_bytes || !backward_bytes) return HV_EINVAL;
-    *saved_bytes = 0;
-    *forward_bytes = attn_workspace(a, false, nullptr).bytes;
-    *backward_bytes = attn_workspace(a, true, nullptr).bytes;
+    if (attn_short(a)) {
+        const ShortPlan p = short_plan(a, true);
+        *saved_bytes = *forward_bytes = 0;
+        *backward_bytes = (size_t)short_blocks(p, a->batch, short_resident(p)) * attn_classes(a) * a->heads * 4;
+        return HV_OK;
+    }
+    LongArgs l = {};
+    float* partial;
+    *saved_bytes = long_saved(a, nullptr, true, &l);
+    *forward_bytes = long_saved(a, nullptr, false, &l);
+    *backward_bytes = long_workspace(a, nullptr, &l, &partial);
     return HV_OK;
 }
 
 int hv_relative_attention_forward(const hv_attention* a, void* out, void* saved, void* workspace, size_t workspace_bytes,
                                   void* stream) {
-    (void)saved;
-    if (!attn_ok(a)) return HV_EINVAL;
-    if (a->batch == 0 || a->queries == 0) return HV_OK;
-    const AttnWorkspace w = attn_workspace(a, false, workspace);
-    if (!out || (w.bytes && (!workspace || !aligned(workspace, 256))) || workspace_bytes < w.bytes) return HV_EINVAL;
+    size_t need[3];
+    const int rc = hv_relative_attention_sizes(a, need, need + 1, need + 2);
+    if (rc) return rc;
+    if (a->batch == 0 || a->tokens == 0 || (a->queries == 0 && !saved)) return HV_OK;
+    // with a saved buffer nothing else is needed
+    if (saved) need[1] = 0;
+    if ((!out && a->queries) || !aligned(saved, 256)) return HV_EINVAL;
+    if (need[1] && (!workspace || !aligned(workspace, 256) || workspace_bytes < need[1])) return HV_EINVAL;
+    const int e = (int)elem_bytes(a->dtype);
+    const cudaStream_t st = (cudaStream_t)stream;
     AttnArgs x = attn_args(a);
-    x.out = out, x.p = w.p;
+    x.out = out;
     x.gs[0] = (int64_t)x.Nq * x.H * x.D, x.gs[1] = (int64_t)x.H * x.D, x.gs[2] = x.D;
     if (attn_short(a)) {
+        if (a->queries == 0) return HV_OK;
         ShortPlan p = short_plan(a, false);
-        short_vec(x, (int)elem_bytes(a->dtype), false, &p);
-        return by_type(a->dtype, [&](auto t) { return launch_short<decltype(t), false>(x, p, (cudaStream_t)stream); });
+        p.vec_in = vec_in(x, e, false), p.vec_out = vec_out(x, e, false);
+        return by_type(a->dtype, [&](auto t) { return launch_short<decltype(t), false>(x, p, st); });
     }
-    const int64_t grid = (x.B * x.H * x.Nq + 3) / 4;
-    if (grid > 0x7fffffff) return HV_EINVAL;
-    return by_type(a->dtype, [&](auto t) {
-        k_attn_row<decltype(t), false><<<(unsigned)grid, 128, 0, (cudaStream_t)stream>>>(x);
-        return launched();
-    });
+    LongArgs l = {};
+    long_saved(a, saved ? saved : workspace, saved != nullptr, &l);
+    l.vec_in = vec_in(x, e, false);
+    if (x.B > 0x7fffffff) return HV_EINVAL;
+    k_attn_sort<<<(unsigned)x.B, x.N <= 256 ? 256 : 1024, 0, st>>>(x, l);
+    if (launched()) return HV_ECUDA;
+    return by_type(a->dtype, [&](auto t) { return launch_long<decltype(t), false>(x, l, st); });
 }
 
 int hv_relative_attention_backward(const hv_attention* a, const void* dout, const int64_t* dout_stride, const void* saved,
                                    void* dq, void* dk, void* dv, const int64_t* dq_stride, const int64_t* dkv_stride,
                                    void* ddq_bias, void* ddr_bias, void* ddz_bias, void* workspace, size_t workspace_bytes,
                                    void* stream) {
-    (void)saved;
-    if (!attn_ok(a) || !ddq_bias || !ddr_bias || !ddz_bias) return HV_EINVAL;
-    const bool empty = a->batch == 0 || a->queries == 0;
-    if (a->batch && a->tokens && (!dk || !dv || !dkv_stride)) return HV_EINVAL;
-    if (!empty && (!dout || !dout_stride || !dq || !dq_stride)) return HV_EINVAL;
-    const AttnWorkspace w = attn_workspace(a, true, workspace);
-    if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.bytes) return HV_EINVAL;
+    size_t need[3];
+    const int rc = hv_relative_attention_sizes(a, need, need + 1, need + 2);
+    if (rc) return rc;
+    if (!ddq_bias || !ddr_bias || !ddz_bias) return HV_EINVAL;
+    if (a->batch && a->tokens && (!dk || !dv || !dkv_stride || (need[0] && !saved))) return HV_EINVAL;
+    if (a->batch && a->queries && (!dout || !dout_stride || !dq || !dq_stride)) return HV_EINVAL;
+    if (need[2] && (!workspace || !aligned(workspace, 256) || workspace_bytes < need[2])) return HV_EINVAL;
+    const int e = (int)elem_bytes(a->dtype);
+    const cudaStream_t st = (cudaStream_t)stream;
     AttnArgs x = attn_args(a);
-    x.dout = dout, x.dq = dq, x.dk = dk, x.dv = dv, x.p = w.p, x.ds = w.ds, x.partial = w.partial;
+    x.dout = dout, x.dq = dq, x.dk = dk, x.dv = dv;
+    x.dbq = ddq_bias, x.dbr = ddr_bias, x.dbz = ddz_bias;
     for (int i = 0; i < 3; i++) {
         x.os[i] = dout_stride ? dout_stride[i] : 0, x.gs[i] = dq_stride ? dq_stride[i] : 0;
         x.gks[i] = dkv_stride ? dkv_stride[i] : 0;
     }
-    x.dbq = ddq_bias, x.dbr = ddr_bias, x.dbz = ddz_bias;
     if (attn_short(a)) {
         ShortPlan p = short_plan(a, true);
-        short_vec(x, (int)elem_bytes(a->dtype), true, &p);
-        return by_type(a->dtype, [&](auto t) { return launch_short<decltype(t), true>(x, p, (cudaStream_t)stream); });
+        p.vec_in = vec_in(x, e, true), p.vec_out = vec_out(x, e, true);
+        x.partial = static_cast<float*>(workspace);
+        return by_type(a->dtype, [&](auto t) { return launch_short<decltype(t), true>(x, p, st); });
     }
-    const int64_t rows = (x.B * x.H * x.Nq + 3) / 4, keys = (x.B * x.H * x.N + 3) / 4;
-    if (rows > 0x7fffffff || keys > 0x7fffffff) return HV_EINVAL;
-    const cudaStream_t st = (cudaStream_t)stream;
-    const int W = 2 * x.clip + 1, classes = attn_classes(a), shares = attn_shares(a);
-    return by_type(a->dtype, [&](auto t) {
-        using T = decltype(t);
-        int rc;
-        if (rows) {
-            k_attn_row<T, true><<<(unsigned)rows, 128, 0, st>>>(x);
-            if ((rc = launched())) return rc;
-        }
-        if (keys) {
-            k_attn_key<T><<<(unsigned)keys, 128, 0, st>>>(x);
-            if ((rc = launched())) return rc;
-        }
-        k_attn_table<<<dim3(shares, x.H), 32, classes * 128, st>>>(x);
-        if ((rc = launched())) return rc;
-        k_attn_table_sum<T><<<(classes * x.H + 3) / 4, 128, 0, st>>>(x.partial, shares, W, classes, x.H, ddq_bias, ddr_bias,
-                                                                    ddz_bias, x.t_f32);
-        return launched();
-    });
+    LongArgs l = {};
+    long_saved(a, const_cast<void*>(saved), true, &l);
+    long_workspace(a, workspace, &l, &x.partial);
+    l.vec_in = vec_in(x, e, true);
+    return by_type(a->dtype, [&](auto t) { return launch_long<decltype(t), true>(x, l, st); });
 }
 
 }  // extern "C"
