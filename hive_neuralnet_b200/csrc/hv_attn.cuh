@@ -12,6 +12,7 @@
 // its output row and its gradients are zero.
 #pragma once
 
+#include "../../include/hive_b200.h"
 #include "hv_elem.cuh"
 
 namespace hv {

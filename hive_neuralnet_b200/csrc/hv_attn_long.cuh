@@ -21,7 +21,6 @@
 namespace hv {
 
 constexpr int kTile = 64;          // tokens of a tile
-constexpr int kLongThreads = 128;
 constexpr float kLog2E = 1.4426950408889634f;
 
 struct LongArgs {
@@ -31,7 +30,7 @@ struct LongArgs {
     float* o32;    // [B][H][Qpad][D], the output before rounding, by slot
     float* delta;  // [B][H][Qpad]
     int Npad, Qpad, tiles;  // tiles: query (key) tiles of a head
-    int vec_in;
+    int vec_in, vec_out;  // 16-byte loads; results stored in pairs
 };
 
 // Row length of a tile in shared memory: an odd number of 16-byte (fp32: 32-byte) units.
@@ -78,82 +77,75 @@ __global__ void __launch_bounds__(1024) k_attn_sort(const AttnArgs a, const Long
     for (int j = a.N + threadIdx.x; j < l.Npad; j += blockDim.x) meta[j] = make_int4(0, 0, 0, 0);
 }
 
-// Rows of a tile, gathered by token.  Rows at or past `end` are zero.
-template <typename T, int DP, int ROWS>
+// Rows of a tile, gathered by token; those at or past `end`, and columns past
+// D, are zero.  With vec, whole 16-byte pieces, asynchronously.
+template <typename T, int DP, int ROWS, int THREADS>
 __device__ __forceinline__ void load_tile(T* dst, const T* src, int64_t stride, int D, const int4* meta, int end, bool vec) {
-    constexpr int LD = tile_ld<T, DP>(), E = 16 / sizeof(T);
+    constexpr int LD = tile_ld<T, DP>(), E = 16 / sizeof(T), PIECES = DP / E, STEP = THREADS / PIECES;
     if (vec) {
-        const int pieces = D / E, rows = kLongThreads / pieces, r0 = threadIdx.x / pieces, x = threadIdx.x - r0 * pieces;
-        if (r0 >= rows) return;
-        for (int r = r0; r < ROWS; r += rows) {
-            T* d = dst + r * LD + x * E;
-            if (r < end)
-                cp_async16(d, src + meta[r].w * stride + x * E);
-            else
-                *reinterpret_cast<uint4*>(d) = make_uint4(0, 0, 0, 0);
-        }
+        const int r0 = threadIdx.x / PIECES, x = threadIdx.x % PIECES * E;
+#pragma unroll
+        for (int r = r0; r < ROWS; r += STEP)
+            cp_async16_or_zero(dst + r * LD + x, src + meta[r].w * stride + x, r < end && x < D);
     } else {
-        for (int i = threadIdx.x; i < ROWS * D; i += kLongThreads) {
-            const int r = i / D, d = i - r * D;
-            dst[r * LD + d] = r < end ? src[meta[r].w * stride + d] : from_f32<T>(0.f);
+        for (int i = threadIdx.x; i < ROWS * DP; i += THREADS) {
+            const int r = i / DP, d = i % DP;
+            dst[r * LD + d] = r < end && d < D ? src[meta[r].w * stride + d] : from_f32<T>(0.f);
         }
     }
 }
+
+// A head's bias (times log2 e) at the start of shared memory, where an entry's
+// address is its class: dq and dz in one table [dz][dq], dr in a second one.
+constexpr int kTabR = 300, kTabBytes = 1344;
+static_assert((2 * HV_ATTN_MAX_HEIGHT_CLIP + 1) * (2 * HV_ATTN_MAX_CLIP + 1) <= kTabR &&
+              (kTabR + 2 * HV_ATTN_MAX_CLIP + 1) * 4 <= kTabBytes && kTabBytes % 16 == 0, "bias tables");
 
 template <typename T>
-__device__ __forceinline__ void load_bias_table(float* tab, const AttnArgs& a, int h) {
-    const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
-    for (int c = threadIdx.x; c < classes; c += kLongThreads) {
-        const void* src = c < W ? a.bq : c < 2 * W ? a.br : a.bz;
-        tab[c] = kLog2E * load_param<T>(src, (int64_t)(c < W ? c : c < 2 * W ? c - W : c - 2 * W) * a.H + h, a.t_f32);
+__device__ __forceinline__ void load_bias_table(char* smem, const AttnArgs& a, int h) {
+    float* tab = reinterpret_cast<float*>(smem);
+    const int W = 2 * a.clip + 1, Z = 2 * a.clip_z + 1;
+    for (int i = threadIdx.x; i < (Z + 1) * W; i += blockDim.x) {
+        const int z = i / W, c = i - z * W;
+        if (z < Z)
+            tab[i] = kLog2E * (load_param<T>(a.bq, (int64_t)c * a.H + h, a.t_f32) + load_param<T>(a.bz, (int64_t)z * a.H + h, a.t_f32));
+        else
+            tab[kTabR + c] = kLog2E * load_param<T>(a.br, (int64_t)c * a.H + h, a.t_f32);
     }
 }
 
-// The bias of a pair, and where its three classes are.
-struct BiasOf {
-    const char *q, *r, *z;
-    int top, top_z;
-    __device__ BiasOf(const float* tab, const AttnArgs& a) {
-        const int W = 2 * a.clip + 1;
-        q = reinterpret_cast<const char*>(tab), r = q + 4 * W, z = q + 8 * W, top = 8 * a.clip, top_z = 8 * a.clip_z;
+// A pair's classes, times 4: from 4 x the key's coordinates and 4 x (clip less
+// the query's).
+struct Classes {
+    int top, top_z, W, q, r, z;
+    __device__ explicit Classes(const AttnArgs& a) : top(8 * a.clip), top_z(8 * a.clip_z), W(2 * a.clip + 1), q(0), r(0), z(0) {}
+    __device__ __forceinline__ void of(int kq, int kr, int kz, int qq, int qr, int qz) {
+        q = __viaddmin_s32_relu(kq, qq, top), r = __viaddmin_s32_relu(kr, qr, top), z = __viaddmin_s32_relu(kz, qz, top_z);
     }
-    __device__ __forceinline__ static float at(const char* p, int c) { return *reinterpret_cast<const float*>(p + c); }
-    // kq, kr, kz: the key's coordinates; qq, qr, qz: 4 clip less the query's
-    __device__ __forceinline__ void classes(int kq, int kr, int kz, int qq, int qr, int qz, int& cq, int& cr, int& cz) const {
-        cq = __viaddmin_s32_relu(kq, qq, top), cr = __viaddmin_s32_relu(kr, qr, top), cz = __viaddmin_s32_relu(kz, qz, top_z);
-    }
-    __device__ __forceinline__ float value(int cq, int cr, int cz) const { return at(q, cq) + at(r, cr) + at(z, cz); }
 };
 
-template <typename T, int DP>
-struct LongSmem {
-    static constexpr int LD = tile_ld<T, DP>();
-    static constexpr int kTileBytes = kTile * LD * (int)sizeof(T);
-    static constexpr int kMetaBytes = kTile * 16;
-};
+__device__ __forceinline__ float bias_of(const char* smem, const Classes& c) {
+    return *reinterpret_cast<const float*>(smem + (c.z * c.W + c.q)) + *reinterpret_cast<const float*>(smem + c.r + kTabR * 4);
+}
 
-// BACK false: the forward pass; true: dq (and delta).  ROWS: 64, or 16 with
-// the keys of each tile shared by the warps.
-template <typename T, int DP, int ROWS, bool BACK>
-__global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, const LongArgs l) {
+// BACK false: the forward pass; true: dq (and delta).  A warp takes 16 of the
+// ROWS queries and 1 / WK of each tile's keys.
+template <typename T, int DP, int ROWS, int WK, bool BACK>
+__global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
-    using S = LongSmem<T, DP>;
-    constexpr int LD = S::LD, NC = DP / 8;
-    constexpr bool SHARED = ROWS == 16;
-    constexpr int NT = SHARED ? 2 : 8;  // 8-key tiles of a warp
-    // The output before rounding gives the backward pass sum_j p dp, which it
-    // takes from every dp: 16-bit probabilities go into it in two parts.  The
-    // score gradients of the backward pass are rounded to the operands' type,
-    // like the results that they are summed into.
-    constexpr bool EXACT = !BACK && sizeof(T) == 2;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = ROWS * 2 * WK;
+    constexpr int NT = 8 / WK;          // 8-key tiles of a warp
+    constexpr int NB = NT < 4 ? NT : 4;
+    // The output before rounding gives the backward pass its sum_j p dp, which it
+    // takes from every dp: there the probabilities need all 24 bits.
+    constexpr int PARTS = BACK || sizeof(T) == 4 ? kParts<T> : __is_same(T, __half) ? 2 : 3;
     extern __shared__ __align__(16) char smem[];
-    T* sq = reinterpret_cast<T*>(smem);
+    T* sq = reinterpret_cast<T*>(smem + kTabBytes);
     T* sg = sq + ROWS * LD;
     T* sk = sg + (BACK ? ROWS * LD : 0);  // two stages of k, then of v
     T* sv = sk + 2 * kTile * LD;
     int4* sm = reinterpret_cast<int4*>(sv + 2 * kTile * LD);  // three tiles of key meta
     int4* qm = sm + 3 * kTile;                                // the queries' meta
-    float* tab = reinterpret_cast<float*>(qm + ROWS);
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
@@ -164,48 +156,44 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
     const int64_t head = b * a.H + h;
     T* out = BACK ? static_cast<T*>(a.dq) + b * a.gs[0] + h * a.gs[2] : static_cast<T*>(a.out) + b * a.gs[0] + h * a.gs[2];
 
-    // masked queries: zeros
-    for (int i = threadIdx.x; i < ROWS * a.D; i += kLongThreads) {
-        const int r = i / a.D, d = i - r * a.D;
-        if (r >= nq && q0 + r < a.Nq) out[meta[n + q0 + r - count.y].w * a.gs[1] + d] = from_f32<T>(0.f);
-    }
+    if (nq < ROWS)  // masked queries: zeros
+        for (int i = threadIdx.x; i < ROWS * a.D; i += THREADS) {
+            const int r = i / a.D, d = i - r * a.D;
+            if (r >= nq && q0 + r < a.Nq) out[meta[n + q0 + r - count.y].w * a.gs[1] + d] = from_f32<T>(0.f);
+        }
     if (nq <= 0) return;
 
     const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
     const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2];
     const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2];
     const T* go = BACK ? static_cast<const T*>(a.dout) + b * a.os[0] + h * a.os[2] : nullptr;
-    if (a.D < DP) {  // the columns past D stay zero
-        uint4* z = reinterpret_cast<uint4*>(smem);
-        for (int i = threadIdx.x; i < (int)(reinterpret_cast<char*>(sm) - smem) / 16; i += kLongThreads) z[i] = make_uint4(0, 0, 0, 0);
-    }
-    load_bias_table<T>(tab, a, h);
-    for (int i = threadIdx.x; i < ROWS; i += kLongThreads) qm[i] = meta[min(q0 + i, l.Npad - 1)];
-    for (int i = threadIdx.x; i < kTile; i += kLongThreads) sm[i] = meta[i];
+    for (int i = threadIdx.x; i < ROWS; i += THREADS) qm[i] = meta[min(q0 + i, l.Npad - 1)];
+    for (int i = threadIdx.x; i < kTile; i += THREADS) sm[i] = meta[i];
     __syncthreads();
-    load_tile<T, DP, ROWS>(sq, q, a.qs[1], a.D, qm, nq, l.vec_in);
-    if (BACK) load_tile<T, DP, ROWS>(sg, go, a.os[1], a.D, qm, nq, l.vec_in);
+    load_tile<T, DP, ROWS, THREADS>(sq, q, a.qs[1], a.D, qm, nq, l.vec_in);
+    if (BACK) load_tile<T, DP, ROWS, THREADS>(sg, go, a.os[1], a.D, qm, nq, l.vec_in);
     const int tiles = (n + kTile - 1) / kTile;
     auto issue = [&](int i) {  // keys of tile i, meta of tile i + 1
         if (i < tiles) {
             const int4* m = sm + i % 3 * kTile;
-            load_tile<T, DP, kTile>(sk + (i & 1) * kTile * LD, k, a.ks[1], a.D, m, n - i * kTile, l.vec_in);
-            load_tile<T, DP, kTile>(sv + (i & 1) * kTile * LD, v, a.vs[1], a.D, m, n - i * kTile, l.vec_in);
+            load_tile<T, DP, kTile, THREADS>(sk + (i & 1) * kTile * LD, k, a.ks[1], a.D, m, n - i * kTile, l.vec_in);
+            load_tile<T, DP, kTile, THREADS>(sv + (i & 1) * kTile * LD, v, a.vs[1], a.D, m, n - i * kTile, l.vec_in);
             if (i + 1 < tiles && threadIdx.x < kTile)
                 cp_async16(sm + (i + 1) % 3 * kTile + threadIdx.x, meta + (i + 1) * kTile + threadIdx.x);
         }
         cp_async_commit();
     };
     issue(0);
+    load_bias_table<T>(smem, a, h);
 
-    const int row0 = SHARED ? 0 : warp * 16, key0 = SHARED ? warp * 16 : 0;
-    const BiasOf bias(tab, a);
+    const int part = warp % WK, row0 = warp / WK * 16, key0 = part * (kTile / WK);
     const float scale2 = a.scale * kLog2E;
+    Classes cls(a);
     int qq[2], qr[2], qz[2];
 #pragma unroll
     for (int r = 0; r < 2; r++) {
         const int4 m = qm[row0 + g + 8 * r];
-        qq[r] = 4 * a.clip - m.x, qr[r] = 4 * a.clip - m.y, qz[r] = 4 * a.clip_z - m.z;
+        qq[r] = (cls.top >> 1) - m.x, qr[r] = (cls.top >> 1) - m.y, qz[r] = (cls.top_z >> 1) - m.z;
     }
     float lse[2] = {0.f, 0.f}, delta[2] = {0.f, 0.f};
     if (BACK) {
@@ -222,7 +210,7 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
             }
             delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 1);
             delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 2);
-            if (row < nq && t == 0 && (!SHARED || warp == 0)) l.delta[head * l.Qpad + q0 + row] = delta[r];
+            if (row < nq && t == 0 && part == 0) l.delta[head * l.Qpad + q0 + row] = delta[r];
         }
     }
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[NC][4];
@@ -235,19 +223,16 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
         cp_async_wait<0>();
         __syncthreads();
         issue(i + 1);
-        const T* tk = sk + (i & 1) * kTile * LD + key0 * LD;
-        const T* tv = sv + (i & 1) * kTile * LD + key0 * LD;
+        const T* tk = sk + ((i & 1) * kTile + key0) * LD;
+        const T* tv = sv + ((i & 1) * kTile + key0) * LD;
         const int4* tm = sm + i % 3 * kTile + key0;
         const int left = n - i * kTile - key0;  // valid keys of this warp's part
         float s[NT][4], dp[BACK ? NT : 1][4];
+        if (BACK)
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+            for (int j = 0; j < NT; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s[j][e] = 0.f;
-                if (BACK) dp[j][e] = 0.f;
-            }
-        constexpr int NB = SHARED ? 2 : 4;
+                for (int e = 0; e < 4; e++) dp[j][e] = -delta[e >> 1];
 #pragma unroll
         for (int d = 0; d < DP; d += Op::KD) {
             typename Op::A qa;
@@ -257,7 +242,10 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
                 typename Op::B kb[NB];
                 Op::load_bn(kb, tk + j * 8 * LD + d, LD, lane);
 #pragma unroll
-                for (int x = 0; x < NB; x++) Op::mma_d(s[j + x], qa, kb[x]);
+                for (int x = 0; x < NB; x++) {
+                    if (d == 0) Op::template mma_d<true>(s[j + x], qa, kb[x]);
+                    else Op::mma_d(s[j + x], qa, kb[x]);
+                }
             }
             if constexpr (BACK) {
                 Op::load_a(qa, sg + row0 * LD + d, LD, lane);
@@ -270,29 +258,34 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
                 }
             }
         }
-        float high[2] = {top[0], top[1]};
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int r = e >> 1;
-                int cq, cr, cz;
-                bias.classes(e & 1 ? mb.x : ma.x, e & 1 ? mb.y : ma.y, e & 1 ? mb.z : ma.z, qq[r], qr[r], qz[r], cq, cr, cz);
-                s[j][e] = fmaf(s[j][e], scale2, bias.value(cq, cr, cz));
-                if (8 * j + 2 * t + (e & 1) >= left) s[j][e] = -INFINITY;
-                if (!BACK) high[r] = fmaxf(high[r], s[j][e]);
+                cls.of(e & 1 ? mb.x : ma.x, e & 1 ? mb.y : ma.y, e & 1 ? mb.z : ma.z, qq[r], qr[r], qz[r]);
+                s[j][e] = fmaf(s[j][e], scale2, bias_of(smem, cls));
             }
         }
+        if (left < NT * 8)  // the last tile
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (8 * j + 2 * t + (e & 1) >= left) s[j][e] = -INFINITY;
         if constexpr (!BACK) {
             float base[2];
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], 1));
-                high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], 2));
-                base[r] = high[r] == -INFINITY ? 0.f : high[r];  // no key of this warp's yet
+                float high = top[r];
+#pragma unroll
+                for (int j = 0; j < NT; j++) high = fmaxf(high, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                base[r] = high == -INFINITY ? 0.f : high;  // no key of this warp's yet
                 const float f = exp2_approx(top[r] - base[r]);
-                top[r] = high[r];
+                top[r] = high;
                 sum[r] *= f;
 #pragma unroll
                 for (int c = 0; c < NC; c++) acc[c][2 * r] *= f, acc[c][2 * r + 1] *= f;
@@ -308,21 +301,19 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    s[j][e] = exp2_approx(s[j][e] - lse[e >> 1]) * (dp[j][e] - delta[e >> 1]);
+                for (int e = 0; e < 4; e++) s[j][e] = exp2_approx(s[j][e] - lse[e >> 1]) * dp[j][e];
         }
         const T* tb = BACK ? tk : tv;
 #pragma unroll
         for (int x = 0; x < NT * 8; x += Op::KK) {
-            typename Op::A pa, pb;
+            typename Op::A pa[PARTS];
             Op::a_from_c(pa, s + x / 8);
-            if constexpr (EXACT) Op::a_rest(pb, pa, s + x / 8);
 #pragma unroll
             for (int c = 0; c < NC; c++) {
                 typename Op::B vb;
                 Op::load_bk(vb, tb + x * LD + 8 * c, LD, lane);
-                Op::mma(acc[c], pa, vb);
-                if constexpr (EXACT) Op::mma(acc[c], pb, vb);
+#pragma unroll
+                for (int y = 0; y < PARTS; y++) Op::mma(acc[c], pa[y], vb);
             }
         }
     }
@@ -332,13 +323,12 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
         sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
     }
-    float inv[2] = {a.scale, a.scale};
-    if (SHARED) {
-        // join the warps' parts, in their order, in warp 0
+    if (WK > 1) {
+        // join the key parts of a row, in their order, in the first part's warp
         __syncthreads();
-        float* join = reinterpret_cast<float*>(smem);  // [warp][16 rows][DP + 2]
         constexpr int JL = DP + 2;
-        float* mine = join + warp * 16 * JL;
+        float* join = reinterpret_cast<float*>(smem + kTabBytes);  // [part][ROWS][DP, maximum, sum]
+        float* mine = join + (part * ROWS + row0) * JL;
 #pragma unroll
         for (int r = 0; r < 2; r++) {
 #pragma unroll
@@ -348,17 +338,18 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
             if (t == 0) mine[(g + 8 * r) * JL + DP] = top[r], mine[(g + 8 * r) * JL + DP + 1] = sum[r];
         }
         __syncthreads();
-        if (warp) return;
+        if (part) return;
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            const float* p = join + (g + 8 * r) * JL;
-            float high = -INFINITY, w[4];
-            for (int x = 0; x < 4; x++) high = fmaxf(high, p[x * 16 * JL + DP]);
+            const float* p = join + (row0 + g + 8 * r) * JL;
+            float high = -INFINITY, w[WK];
+#pragma unroll
+            for (int x = 0; x < WK; x++) high = fmaxf(high, p[x * ROWS * JL + DP]);
             sum[r] = 0.f;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                w[x] = BACK ? 1.f : exp2_approx(p[x * 16 * JL + DP] - high);
-                sum[r] += w[x] * p[x * 16 * JL + DP + 1];
+            for (int x = 0; x < WK; x++) {
+                w[x] = BACK ? 1.f : exp2_approx(p[x * ROWS * JL + DP] - high);
+                sum[r] += w[x] * p[x * ROWS * JL + DP + 1];
             }
             top[r] = high;
 #pragma unroll
@@ -367,7 +358,7 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
                 for (int e = 0; e < 2; e++) {
                     float z = 0.f;
 #pragma unroll
-                    for (int x = 0; x < 4; x++) z = fmaf(w[x], p[x * 16 * JL + 8 * c + 2 * t + e], z);
+                    for (int x = 0; x < WK; x++) z = fmaf(w[x], p[x * ROWS * JL + 8 * c + 2 * t + e], z);
                     acc[c][2 * r + e] = z;
                 }
         }
@@ -377,45 +368,52 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_query(const AttnArgs a, c
         const int row = row0 + g + 8 * r;
         if (row >= nq) continue;
         const int64_t at = head * l.Qpad + q0 + row;
-        if (!BACK) {
-            inv[r] = 1.f / sum[r];
-            if (l.lse && t == 0) l.lse[at] = top[r] + log2f(sum[r]);
-        }
+        if (!BACK && l.lse && t == 0) l.lse[at] = top[r] + log2f(sum[r]);
+        const float f = BACK ? a.scale : 1.f / sum[r];
         T* dst = out + qm[row].w * a.gs[1];
 #pragma unroll
-        for (int c = 0; c < NC; c++)
+        for (int c = 0; c < NC; c++) {
+            const int d = 8 * c + 2 * t;
+            const float o[2] = {acc[c][2 * r] * f, acc[c][2 * r + 1] * f};
+            if (l.vec_out) {  // D is even
+                if (d < a.D) {
+                    store_vec<T, 2>(dst + d, o);
+                    if (!BACK && l.o32) store_vec<float, 2>(l.o32 + at * a.D + d, o);
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int d = 8 * c + 2 * t + e;
-                if (d >= a.D) continue;
-                const float o = acc[c][2 * r + e] * inv[r];
-                dst[d] = from_f32<T>(o);
-                if (!BACK && l.o32) l.o32[at * a.D + d] = o;
+                for (int e = 0; e < 2; e++)
+                    if (d + e < a.D) {
+                        dst[d + e] = from_f32<T>(o[e]);
+                        if (!BACK && l.o32) l.o32[at * a.D + d + e] = o[e];
+                    }
             }
+        }
     }
 }
 
-// dk, dv and the bias sums of 64 keys of one head.
-template <typename T, int DP>
-__global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, const LongArgs l) {
+// dk, dv and the bias sums of 64 keys of one head.  A warp takes 16 of the keys
+// and, of each tile's queries, 32 at a time: all of them in turn, or (WQ = 2)
+// one half.
+template <typename T, int DP, int WQ>
+__global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
-    using S = LongSmem<T, DP>;
-    constexpr int LD = S::LD, NC = DP / 8;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = 128 * WQ, PARTS = kParts<T>;
     extern __shared__ __align__(16) char smem[];
-    T* sk = reinterpret_cast<T*>(smem);
+    T* sk = reinterpret_cast<T*>(smem + kTabBytes);
     T* sv = sk + kTile * LD;
     T* sq = sv + kTile * LD;  // two stages of q, then of dout
     T* sg = sq + 2 * kTile * LD;
     int4* sm = reinterpret_cast<int4*>(sg + 2 * kTile * LD);  // three tiles of query meta
     int4* km = sm + 3 * kTile;                                // the keys' meta
-    float2* sd = reinterpret_cast<float2*>(km + kTile);       // two tiles of (lse, delta)
-    float* tab = reinterpret_cast<float*>(sd + 2 * kTile);
+    float2* sd = reinterpret_cast<float2*>(km + kTile);       // two tiles of (lse, -delta)
+    float* hist = reinterpret_cast<float*>(sd + 2 * kTile);   // [warp][class][lane]
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int key0 = warp % 4 * 16, half = warp / 4;
     const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
     const int64_t b = blockIdx.x / l.tiles / a.H;
     const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
-    float* hist = tab + classes;
     const int2 count = l.count[b];
     const int k0 = tile * kTile, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below 64
     const int4* meta = l.meta + b * l.Npad;
@@ -423,40 +421,35 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, co
     float* part = a.partial + ((b * l.tiles + tile) * classes) * a.H + h;
     T* dk = static_cast<T*>(a.dk) + b * a.gks[0] + h * a.gks[2];
     T* dv = static_cast<T*>(a.dv) + b * a.gks[0] + h * a.gks[2];
-    for (int i = threadIdx.x; i < kTile * a.D; i += kLongThreads) {  // masked keys: zeros
-        const int r = i / a.D, d = i - r * a.D;
-        if (r >= n && k0 + r < a.N) {
-            const int64_t at = meta[k0 + r].w * a.gks[1] + d;
-            dk[at] = dv[at] = from_f32<T>(0.f);
+    if (n < kTile)  // masked keys: zeros
+        for (int i = threadIdx.x; i < kTile * a.D; i += THREADS) {
+            const int r = i / a.D, d = i - r * a.D;
+            if (r >= n && k0 + r < a.N) {
+                const int64_t at = meta[k0 + r].w * a.gks[1] + d;
+                dk[at] = dv[at] = from_f32<T>(0.f);
+            }
         }
-    }
     if (n <= 0) {
-        for (int c = threadIdx.x; c < classes; c += kLongThreads) part[(int64_t)c * a.H] = 0.f;
+        for (int c = threadIdx.x; c < classes; c += THREADS) part[(int64_t)c * a.H] = 0.f;
         return;
     }
     const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
     const T* go = static_cast<const T*>(a.dout) + b * a.os[0] + h * a.os[2];
-    if (a.D < DP) {
-        uint4* z = reinterpret_cast<uint4*>(smem);
-        for (int i = threadIdx.x; i < (int)(reinterpret_cast<char*>(sm) - smem) / 16; i += kLongThreads) z[i] = make_uint4(0, 0, 0, 0);
-    }
-    load_bias_table<T>(tab, a, h);
-    for (int i = threadIdx.x; i < classes * kLongThreads; i += kLongThreads) hist[i] = 0.f;
-    for (int i = threadIdx.x; i < kTile; i += kLongThreads) km[i] = meta[k0 + i], sm[i] = meta[i];
+    for (int i = threadIdx.x; i < kTile; i += THREADS) km[i] = meta[k0 + i], sm[i] = meta[i];
     __syncthreads();
-    load_tile<T, DP, kTile>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
-    load_tile<T, DP, kTile>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, kTile, THREADS>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, kTile, THREADS>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
     const int tiles = (nq + kTile - 1) / kTile;
     auto issue = [&](int i) {
         if (i < tiles) {
             const int4* m = sm + i % 3 * kTile;
-            load_tile<T, DP, kTile>(sq + (i & 1) * kTile * LD, q, a.qs[1], a.D, m, nq - i * kTile, l.vec_in);
-            load_tile<T, DP, kTile>(sg + (i & 1) * kTile * LD, go, a.os[1], a.D, m, nq - i * kTile, l.vec_in);
+            load_tile<T, DP, kTile, THREADS>(sq + (i & 1) * kTile * LD, q, a.qs[1], a.D, m, nq - i * kTile, l.vec_in);
+            load_tile<T, DP, kTile, THREADS>(sg + (i & 1) * kTile * LD, go, a.os[1], a.D, m, nq - i * kTile, l.vec_in);
             if (threadIdx.x < kTile) {
                 const int s = i * kTile + threadIdx.x;
                 // past the last query: a probability of zero
                 float2 x = make_float2(INFINITY, 0.f);
-                if (s < nq) x = make_float2(l.lse[head * l.Qpad + s], l.delta[head * l.Qpad + s]);
+                if (s < nq) x = make_float2(l.lse[head * l.Qpad + s], -l.delta[head * l.Qpad + s]);
                 sd[(i & 1) * kTile + threadIdx.x] = x;
                 if (i + 1 < tiles)
                     cp_async16(sm + (i + 1) % 3 * kTile + threadIdx.x, meta + (i + 1) * kTile + threadIdx.x);
@@ -465,16 +458,18 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, co
         cp_async_commit();
     };
     issue(0);
-    const BiasOf bias(tab, a);
+    load_bias_table<T>(smem, a, h);
+    for (int i = threadIdx.x; i < classes * THREADS; i += THREADS) hist[i] = 0.f;
     const float scale2 = a.scale * kLog2E;
     char* sums = reinterpret_cast<char*>(hist + warp * classes * 32 + lane);
+    Classes cls(a);
     int kq[2], kr[2], kz[2];
     bool live[2];
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-        const int4 m = km[warp * 16 + g + 8 * r];
-        kq[r] = m.x + 4 * a.clip, kr[r] = m.y + 4 * a.clip, kz[r] = m.z + 4 * a.clip_z;
-        live[r] = warp * 16 + g + 8 * r < n;
+        const int4 m = km[key0 + g + 8 * r];
+        kq[r] = m.x + (cls.top >> 1), kr[r] = m.y + (cls.top >> 1), kz[r] = m.z + (cls.top_z >> 1);
+        live[r] = key0 + g + 8 * r < n;
     }
     float ak[NC][4], av[NC][4];
 #pragma unroll
@@ -487,26 +482,30 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, co
         __syncthreads();
         issue(i + 1);
 #pragma unroll 1
-        for (int y = 0; y < kTile; y += 32) {  // 32 queries at a time
-            if (i * kTile + y >= nq) break;
+        for (int y = 32 * half; y < kTile; y += 32 * WQ) {
+            if (i * kTile + y >= nq || key0 >= n) break;
             const T* tq = sq + ((i & 1) * kTile + y) * LD;
             const T* tg = sg + ((i & 1) * kTile + y) * LD;
             const int4* tm = sm + i % 3 * kTile + y;
             const float2* td = sd + (i & 1) * kTile + y;
             float s[4][4], dp[4][4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[j][e] = dp[j][e] = 0.f;
+            for (int j = 0; j < 4; j++) {
+                const float4 x = *reinterpret_cast<const float4*>(td + 8 * j + 2 * t);
+                dp[j][0] = dp[j][2] = x.y, dp[j][1] = dp[j][3] = x.w;
+            }
 #pragma unroll
             for (int d = 0; d < DP; d += Op::KD) {
                 typename Op::A ka;
                 typename Op::B qb[4];
-                Op::load_a(ka, sk + warp * 16 * LD + d, LD, lane);
+                Op::load_a(ka, sk + key0 * LD + d, LD, lane);
                 Op::load_bn(qb, tq + d, LD, lane);
 #pragma unroll
-                for (int x = 0; x < 4; x++) Op::mma_d(s[x], ka, qb[x]);
-                Op::load_a(ka, sv + warp * 16 * LD + d, LD, lane);
+                for (int x = 0; x < 4; x++) {
+                    if (d == 0) Op::template mma_d<true>(s[x], ka, qb[x]);
+                    else Op::mma_d(s[x], ka, qb[x]);
+                }
+                Op::load_a(ka, sv + key0 * LD + d, LD, lane);
                 Op::load_bn(qb, tg + d, LD, lane);
 #pragma unroll
                 for (int x = 0; x < 4; x++) Op::mma_d(dp[x], ka, qb[x]);
@@ -514,19 +513,17 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, co
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
-                const float2 da = td[8 * j + 2 * t], db = td[8 * j + 2 * t + 1];
+                const float4 x = *reinterpret_cast<const float4*>(td + 8 * j + 2 * t);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int r = e >> 1;
-                    int cq, cr, cz;
-                    bias.classes(kq[r], kr[r], kz[r], -(e & 1 ? mb.x : ma.x), -(e & 1 ? mb.y : ma.y), -(e & 1 ? mb.z : ma.z), cq,
-                                 cr, cz);
-                    const float x = fmaf(s[j][e], scale2, bias.value(cq, cr, cz));
-                    s[j][e] = live[r] ? exp2_approx(x - (e & 1 ? db.x : da.x)) : 0.f;
-                    dp[j][e] = s[j][e] * (dp[j][e] - (e & 1 ? db.y : da.y));
-                    float* hq = reinterpret_cast<float*>(sums + cq * 32);
-                    float* hr = reinterpret_cast<float*>(sums + W * 128 + cr * 32);
-                    float* hz = reinterpret_cast<float*>(sums + 2 * W * 128 + cz * 32);
+                    cls.of(kq[r], kr[r], kz[r], -(e & 1 ? mb.x : ma.x), -(e & 1 ? mb.y : ma.y), -(e & 1 ? mb.z : ma.z));
+                    const float y2 = fmaf(s[j][e], scale2, bias_of(smem, cls));
+                    s[j][e] = live[r] ? exp2_approx(y2 - (e & 1 ? x.z : x.x)) : 0.f;
+                    dp[j][e] *= s[j][e];
+                    float* hq = reinterpret_cast<float*>(sums + cls.q * 32);
+                    float* hr = reinterpret_cast<float*>(sums + W * 128 + cls.r * 32);
+                    float* hz = reinterpret_cast<float*>(sums + 2 * W * 128 + cls.z * 32);
                     const float xq = *hq, xr = *hr, xz = *hz;
                     *hq = xq + dp[j][e];
                     *hr = xr + dp[j][e];
@@ -535,42 +532,69 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, co
             }
 #pragma unroll
             for (int x = 0; x < 32; x += Op::KK) {
-                typename Op::A pa;
+                typename Op::A pa[PARTS];
                 Op::a_from_c(pa, s + x / 8);
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     typename Op::B gb;
                     Op::load_bk(gb, tg + x * LD + 8 * c, LD, lane);
-                    Op::mma(av[c], pa, gb);
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) Op::mma(av[c], pa[p], gb);
                 }
                 Op::a_from_c(pa, dp + x / 8);
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     typename Op::B qb;
                     Op::load_bk(qb, tq + x * LD + 8 * c, LD, lane);
-                    Op::mma(ak[c], pa, qb);
+#pragma unroll
+                    for (int p = 0; p < PARTS; p++) Op::mma(ak[c], pa[p], qb);
                 }
             }
         }
     }
     cp_async_wait<0>();
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int row = warp * 16 + g + 8 * r;
-        if (row >= n) continue;
-        const int64_t at = km[row].w * a.gks[1];
-#pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int d = 8 * c + 2 * t + e;
-                if (d >= a.D) continue;
-                dk[at + d] = from_f32<T>(ak[c][2 * r + e] * a.scale);
-                dv[at + d] = from_f32<T>(av[c][2 * r + e]);
-            }
-    }
-    // this block's sums: a lane a class over its warp's 32 columns, then the warps
     __syncthreads();
+    if (WQ > 1) {  // the halves' sums, first half first
+        float* join = reinterpret_cast<float*>(smem + kTabBytes) + (key0 + g) * 2 * DP + 2 * t;
+        if (half)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    *reinterpret_cast<float2*>(join + r * 16 * DP + 8 * c) = make_float2(ak[c][2 * r], ak[c][2 * r + 1]);
+                    *reinterpret_cast<float2*>(join + r * 16 * DP + DP + 8 * c) = make_float2(av[c][2 * r], av[c][2 * r + 1]);
+                }
+        __syncthreads();
+        if (!half)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const float2 x = *reinterpret_cast<const float2*>(join + r * 16 * DP + 8 * c);
+                    const float2 y = *reinterpret_cast<const float2*>(join + r * 16 * DP + DP + 8 * c);
+                    ak[c][2 * r] += x.x, ak[c][2 * r + 1] += x.y, av[c][2 * r] += y.x, av[c][2 * r + 1] += y.y;
+                }
+    }
+    if (!half)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            const int row = key0 + g + 8 * r;
+            if (row >= n) continue;
+            const int64_t at = km[row].w * a.gks[1];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const int d = 8 * c + 2 * t;
+                const float x[2] = {ak[c][2 * r] * a.scale, ak[c][2 * r + 1] * a.scale}, y[2] = {av[c][2 * r], av[c][2 * r + 1]};
+                if (l.vec_out) {
+                    if (d < a.D) store_vec<T, 2>(dk + at + d, x), store_vec<T, 2>(dv + at + d, y);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        if (d + e < a.D) dk[at + d + e] = from_f32<T>(x[e]), dv[at + d + e] = from_f32<T>(y[e]);
+                }
+            }
+        }
+    // this block's bias sums: a lane a class over its warp's 32 columns, then the warps
     for (int c = lane; c < classes; c += 32) {
         const float* col = hist + (warp * classes + c) * 32;
         float x = 0.f;
@@ -578,9 +602,9 @@ __global__ void __launch_bounds__(kLongThreads) k_attn_keys(const AttnArgs a, co
         hist[(warp * classes + c) * 32] = x;
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < classes; c += kLongThreads) {
+    for (int c = threadIdx.x; c < classes; c += THREADS) {
         float x = 0.f;
-        for (int w = 0; w < 4; w++) x += hist[(w * classes + c) * 32];
+        for (int w = 0; w < 4 * WQ; w++) x += hist[(w * classes + c) * 32];
         part[(int64_t)c * a.H] = x;
     }
 }

@@ -107,7 +107,7 @@ struct ClassOf {
 template <typename T, int DP, bool BACK>
 __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const ShortPlan p) {
     using Op = Tile<T, DP == 8>;
-    constexpr int NC = DP / 8;  // 8-value chunks of a head
+    constexpr int NC = DP / 8, PARTS = kParts<T>;  // 8-value chunks of a head
     constexpr bool F32 = sizeof(T) == 4;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
@@ -292,13 +292,14 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
 #pragma unroll
                     for (int k = 0; k < kSlots; k += Op::KK) {
                         if (k >= n) continue;
-                        typename Op::A pa;
+                        typename Op::A pa[PARTS];
                         Op::a_from_c(pa, s + k / 8);
 #pragma unroll
                         for (int c = 0; c < NC; c++) {
                             typename Op::B vb;
                             Op::load_bk(vb, V + k * ld + 8 * c, ld, lane);
-                            Op::mma(o[c], pa, vb);
+#pragma unroll
+                            for (int x = 0; x < PARTS; x++) Op::mma(o[c], pa[x], vb);
                         }
                     }
                     __syncwarp();
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                             *hz = xz + dp[i][e];
                         }
                     }
-                    typename Op::A pt[2][16 / Op::KK];
+                    typename Op::A pt[PARTS][2][16 / Op::KK];
                     float* room = scratch + (F32 ? warp * 16 * kTransposeLd : 0);
                     transpose_c<T, DP == 8>(pt, s, room, lane);
 #pragma unroll
@@ -353,8 +354,11 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                         for (int c = 0; c < NC; c++) {
                             typename Op::B gb;
                             Op::load_bk(gb, G + (m0 + k * Op::KK) * ld + 8 * c, ld, lane);
-                            Op::mma(dv[0][c], pt[0][k], gb);
-                            if (n > 16) Op::mma(dv[1][c], pt[1][k], gb);
+#pragma unroll
+                            for (int y = 0; y < PARTS; y++) {
+                                Op::mma(dv[0][c], pt[y][0][k], gb);
+                                if (n > 16) Op::mma(dv[1][c], pt[y][1][k], gb);
+                            }
                         }
                     transpose_c<T, DP == 8>(pt, dp, room, lane);
 #pragma unroll
@@ -363,8 +367,11 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                         for (int c = 0; c < NC; c++) {
                             typename Op::B qb;
                             Op::load_bk(qb, Q + (m0 + k * Op::KK) * ld + 8 * c, ld, lane);
-                            Op::mma(dk[0][c], pt[0][k], qb);
-                            if (n > 16) Op::mma(dk[1][c], pt[1][k], qb);
+#pragma unroll
+                            for (int y = 0; y < PARTS; y++) {
+                                Op::mma(dk[0][c], pt[y][0][k], qb);
+                                if (n > 16) Op::mma(dk[1][c], pt[y][1][k], qb);
+                            }
                         }
                     __syncwarp();  // this tile's rows of Q are done with: dq takes their place
 #pragma unroll
@@ -373,11 +380,12 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
 #pragma unroll
                         for (int k = 0; k < kSlots; k += Op::KK) {
                             if (k >= n) continue;
-                            typename Op::A da;
+                            typename Op::A da[PARTS];
                             typename Op::B kb;
                             Op::a_from_c(da, dp + k / 8);
                             Op::load_bk(kb, K + k * ld + 8 * c, ld, lane);
-                            Op::mma(o, da, kb);
+#pragma unroll
+                            for (int y = 0; y < PARTS; y++) Op::mma(o, da[y], kb);
                         }
                         float lo[2] = {o[0] * a.scale, o[1] * a.scale}, hi[2] = {o[2] * a.scale, o[3] * a.scale};
                         store_vec<T, 2>(Q + (m0 + g) * ld + 8 * c + 2 * t, lo);

@@ -10,7 +10,10 @@
 // hi hi + hi lo + lo hi: the dropped lo lo is below 2^-22 of it.
 //
 // Layouts (g = lane / 4, t = lane % 4).  C: c[0..1] row g, c[2..3] row g + 8,
-// columns 2t, 2t + 1.  The order of k inside a step is free as long as both
+// columns 2t, 2t + 1.  Rates measured here
+// (an SM, a clock): mma m16n8k16 of 16-bit types, m16n8k8 of theirs or of tf32
+// 0.48 each, movmatrix 1, ex2 0.5 warp instructions.  The order of k inside a
+// step is free as long as both
 // operands share it; fp32 steps (8 wide) pair k = t, t + 4 with columns 2t,
 // 2t + 1, so a C tile is an A operand without moving a value.
 #pragma once
@@ -56,27 +59,29 @@ __device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 
-#define HV_MMA16(NAME, TYPE)                                                                                          \
-    __device__ __forceinline__ void NAME##_k16(float* c, const uint32_t* a, const uint32_t* b) {                      \
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32." TYPE "." TYPE                                           \
-                     ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                                     \
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                 \
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));                             \
-    }                                                                                                                 \
-    __device__ __forceinline__ void NAME##_k8(float* c, const uint32_t* a, const uint32_t* b) {                       \
-        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32." TYPE "." TYPE ".f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};" \
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                                 \
-                     : "r"(a[0]), "r"(a[1]), "r"(b[0]));                                                              \
+// c = a b + (FIRST ? 0 : c)
+#define HV_MMA(NAME, SHAPE, TYPES, NA, AREGS, BREGS)                                                                    \
+    template <bool FIRST>                                                                                               \
+    __device__ __forceinline__ void NAME(float* c, const uint32_t* a, const uint32_t* b) {                              \
+        if constexpr (FIRST)                                                                                            \
+            asm volatile("mma.sync.aligned." SHAPE ".row.col.f32." TYPES ".f32 {%0,%1,%2,%3}, " AREGS ", " BREGS        \
+                         ", {%10,%10,%10,%10};"                                                                         \
+                         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])                                               \
+                         : "r"(a[0]), "r"(a[1]), "r"(a[NA > 2 ? 2 : 0]), "r"(a[NA > 2 ? 3 : 0]), "r"(b[0]),             \
+                           "r"(b[NA > 2 ? 1 : 0]), "f"(0.f));                                                           \
+        else                                                                                                            \
+            asm volatile("mma.sync.aligned." SHAPE ".row.col.f32." TYPES ".f32 {%0,%1,%2,%3}, " AREGS ", " BREGS        \
+                         ", {%0,%1,%2,%3};"                                                                             \
+                         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])                                               \
+                         : "r"(a[0]), "r"(a[1]), "r"(a[NA > 2 ? 2 : 0]), "r"(a[NA > 2 ? 3 : 0]), "r"(b[0]),             \
+                           "r"(b[NA > 2 ? 1 : 0]));                                                                     \
     }
-HV_MMA16(mma_f16, "f16")
-HV_MMA16(mma_bf16, "bf16")
-#undef HV_MMA16
-
-__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, const uint32_t* b) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
+HV_MMA(mma_f16_k16, "m16n8k16", "f16.f16", 4, "{%4,%5,%6,%7}", "{%8,%9}")
+HV_MMA(mma_f16_k8, "m16n8k8", "f16.f16", 2, "{%4,%5}", "{%8}")
+HV_MMA(mma_bf16_k16, "m16n8k16", "bf16.bf16", 4, "{%4,%5,%6,%7}", "{%8,%9}")
+HV_MMA(mma_bf16_k8, "m16n8k8", "bf16.bf16", 2, "{%4,%5}", "{%8}")
+HV_MMA(mma_tf32, "m16n8k8", "tf32.tf32", 4, "{%4,%5,%6,%7}", "{%8,%9}")
+#undef HV_MMA
 
 // hi: the value rounded to the 11 significant bits of tf32, lo: the rest,
 // rounded likewise (cut off instead, the errors would all have one sign).
@@ -94,14 +99,16 @@ struct Tile {  // 16-bit types
     struct A { uint32_t r[4]; };
     struct B { uint32_t r[2]; };
 
+    template <bool FIRST = false>
     __device__ static void mma(float* c, const A& a, const B& b) {
-        if constexpr (sizeof(T) == 2 && __is_same(T, __half)) mma_f16_k16(c, a.r, b.r);
-        else mma_bf16_k16(c, a.r, b.r);
+        if constexpr (__is_same(T, __half)) mma_f16_k16<FIRST>(c, a.r, b.r);
+        else mma_bf16_k16<FIRST>(c, a.r, b.r);
     }
+    template <bool FIRST = false>
     __device__ static void mma_d(float* c, const A& a, const B& b) {
-        if constexpr (!D8) mma(c, a, b);
-        else if constexpr (__is_same(T, __half)) mma_f16_k8(c, a.r, b.r);
-        else mma_bf16_k8(c, a.r, b.r);
+        if constexpr (!D8) mma<FIRST>(c, a, b);
+        else if constexpr (__is_same(T, __half)) mma_f16_k8<FIRST>(c, a.r, b.r);
+        else mma_bf16_k8<FIRST>(c, a.r, b.r);
     }
     // 16 rows x KD values at p (row-major, ld elements a row)
     __device__ static void load_a(A& a, const T* p, int ld, int lane) {
@@ -131,21 +138,22 @@ struct Tile {  // 16-bit types
     }
     // KK rows x 8 values at p as a B operand (k = row)
     __device__ static void load_bk(B& b, const T* p, int ld, int lane) { ldsm2_t(b.r[0], b.r[1], p + (lane & 15) * ld); }
-    // What a_from_c left of the C tiles, as a second operand: with it a product
-    // has 16 (fp16: 22) bits of them instead of 8 (11).
-    __device__ static void a_rest(A& a, const A& first, const float (*c)[4]) {
+    // C tiles of 16 rows x KK columns as PARTS A operands (k = column): the
+    // values rounded, then what the rounding left, rounded, ...
+    template <int PARTS>
+    __device__ static void a_from_c(A (&a)[PARTS], const float (*c)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float2 f = unpack2(first.r[i], T());
-            a.r[i] = pack2(c[i >> 1][2 * (i & 1)] - f.x, c[i >> 1][2 * (i & 1) + 1] - f.y, T());
+            float x = c[i >> 1][2 * (i & 1)], y = c[i >> 1][2 * (i & 1) + 1];
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) {
+                a[p].r[i] = pack2(x, y, T());
+                if (p + 1 < PARTS) {
+                    const float2 f = unpack2(a[p].r[i], T());
+                    x -= f.x, y -= f.y;
+                }
+            }
         }
-    }
-    // C tiles of 16 rows x KK columns as an A operand (k = column)
-    __device__ static void a_from_c(A& a, const float (*c)[4]) {
-        a.r[0] = pack2(c[0][0], c[0][1], T());
-        a.r[1] = pack2(c[0][2], c[0][3], T());
-        a.r[2] = pack2(c[1][0], c[1][1], T());
-        a.r[3] = pack2(c[1][2], c[1][3], T());
     }
 };
 
@@ -155,12 +163,14 @@ struct Tile<float, D8> {
     struct A { uint32_t hi[4], lo[4]; };
     struct B { uint32_t hi[2], lo[2]; };
 
+    template <bool FIRST = false>
     __device__ static void mma(float* c, const A& a, const B& b) {
-        mma_tf32(c, a.lo, b.hi);
-        mma_tf32(c, a.hi, b.lo);
-        mma_tf32(c, a.hi, b.hi);
+        mma_tf32<FIRST>(c, a.lo, b.hi);
+        mma_tf32<false>(c, a.hi, b.lo);
+        mma_tf32<false>(c, a.hi, b.hi);
     }
-    __device__ static void mma_d(float* c, const A& a, const B& b) { mma(c, a, b); }
+    template <bool FIRST = false>
+    __device__ static void mma_d(float* c, const A& a, const B& b) { mma<FIRST>(c, a, b); }
     __device__ static void load_a(A& a, const float* p, int ld, int lane) {
         const float* q = p + (lane >> 2) * ld + 2 * (lane & 3);
         const float2 x = *reinterpret_cast<const float2*>(q), y = *reinterpret_cast<const float2*>(q + 8 * ld);
@@ -183,30 +193,40 @@ struct Tile<float, D8> {
         split_tf32(q[0], b.hi[0], b.lo[0]);
         split_tf32(q[ld], b.hi[1], b.lo[1]);
     }
-    __device__ static void a_from_c(A& a, const float (*c)[4]) {
-        split_tf32(c[0][0], a.hi[0], a.lo[0]);
-        split_tf32(c[0][2], a.hi[1], a.lo[1]);
-        split_tf32(c[0][1], a.hi[2], a.lo[2]);
-        split_tf32(c[0][3], a.hi[3], a.lo[3]);
+    __device__ static void a_from_c(A (&a)[1], const float (*c)[4]) {
+        split_tf32(c[0][0], a[0].hi[0], a[0].lo[0]);
+        split_tf32(c[0][2], a[0].hi[1], a[0].lo[1]);
+        split_tf32(c[0][1], a[0].hi[2], a[0].lo[2]);
+        split_tf32(c[0][3], a[0].hi[3], a[0].lo[3]);
     }
 };
 
+// In how many parts of the operands' type the probabilities and the score
+// gradients go into a product: rounded to 8 (11) bits once, their errors would
+// be as large in the results as the results' own rounding.  Two parts hold 16
+// (22) bits.  fp32 operands are split by the product itself.
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 1 : 2;
+
 // The transpose of 16 x 32 C tiles (rows: queries, columns: keys) as A operands
-// [2][16 / KK] (m = key, k = query): in registers for 16-bit types, through
-// 16 x kTransposeLd floats of the warp's own for fp32.
+// [part][2][16 / KK] (m = key, k = query): in registers for 16-bit types,
+// through 16 x kTransposeLd floats of the warp's own for fp32.
 constexpr int kTransposeLd = 36;
 
 template <typename T, bool D8>
-__device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[2][16 / Tile<T, D8>::KK], const float (&c)[4][4],
-                                            float* scratch, int lane) {
+__device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[kParts<T>][2][16 / Tile<T, D8>::KK],
+                                            const float (&c)[4][4], float* scratch, int lane) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
-            a[m][0].r[0] = transpose8(pack2(c[2 * m][0], c[2 * m][1], T()));
-            a[m][0].r[1] = transpose8(pack2(c[2 * m + 1][0], c[2 * m + 1][1], T()));
-            a[m][0].r[2] = transpose8(pack2(c[2 * m][2], c[2 * m][3], T()));
-            a[m][0].r[3] = transpose8(pack2(c[2 * m + 1][2], c[2 * m + 1][3], T()));
-        }
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float* v = c[2 * m + (i & 1)] + 2 * (i >> 1);
+                const uint32_t first = pack2(v[0], v[1], T());
+                const float2 f = unpack2(first, T());
+                a[0][m][0].r[i] = transpose8(first);
+                a[1][m][0].r[i] = transpose8(pack2(v[0] - f.x, v[1] - f.y, T()));
+            }
     } else {
         const int g = lane >> 2, t = lane & 3;
         __syncwarp();
@@ -221,16 +241,21 @@ __device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[2][16 /
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const float* p = scratch + (8 * k + 2 * t) * kTransposeLd + 16 * m + g;
-                split_tf32(p[0], a[m][k].hi[0], a[m][k].lo[0]);
-                split_tf32(p[8], a[m][k].hi[1], a[m][k].lo[1]);
-                split_tf32(p[kTransposeLd], a[m][k].hi[2], a[m][k].lo[2]);
-                split_tf32(p[kTransposeLd + 8], a[m][k].hi[3], a[m][k].lo[3]);
+                auto& x = a[0][m][k];
+                split_tf32(p[0], x.hi[0], x.lo[0]);
+                split_tf32(p[8], x.hi[1], x.lo[1]);
+                split_tf32(p[kTransposeLd], x.hi[2], x.lo[2]);
+                split_tf32(p[kTransposeLd + 8], x.hi[3], x.lo[3]);
             }
     }
 }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+// 16 bytes, or 16 zero bytes (the source is not read)
+__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool read) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(read ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

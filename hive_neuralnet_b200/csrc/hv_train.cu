@@ -259,39 +259,33 @@ static size_t long_workspace(const hv_attention* a, void* base, LongArgs* l, flo
     return delta + (size_t)blocks * attn_classes(a) * a->heads * 4;
 }
 
-// 16 queries a block where blocks of 64 would leave SMs without one.
-static bool few_queries(const AttnArgs& x) {
-    return x.Nq <= 16 || x.B * x.H * ((x.Nq + kTile - 1) / kTile) < sm_count();
-}
-
-template <typename T, int DP, int ROWS, bool BACK>
+template <typename T, int DP, int ROWS, int WK, bool BACK>
 static int launch_query(const AttnArgs& x, LongArgs l, cudaStream_t st) {
-    constexpr int LD = tile_ld<T, DP>();
-    const int classes = 2 * (2 * x.clip + 1) + 2 * x.clip_z + 1;
-    const int smem = (ROWS * (BACK ? 2 : 1) + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + ROWS) * 16 + classes * 4;
+    constexpr int LD = tile_ld<T, DP>(), threads = ROWS * 2 * WK;
+    const int smem = kTabBytes + (ROWS * (BACK ? 2 : 1) + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + ROWS) * 16;
     l.tiles = (x.Nq + ROWS - 1) / ROWS;
     const int64_t grid = x.B * x.H * l.tiles;
     if (grid > 0x7fffffff) return HV_EINVAL;
     int n = 0;
-    const int rc = resident_blocks(k_attn_query<T, DP, ROWS, BACK>, kLongThreads, smem, &n);
+    const int rc = resident_blocks(k_attn_query<T, DP, ROWS, WK, BACK>, threads, smem, &n);
     if (rc) return rc;
-    k_attn_query<T, DP, ROWS, BACK><<<(unsigned)grid, kLongThreads, smem, st>>>(x, l);
+    k_attn_query<T, DP, ROWS, WK, BACK><<<(unsigned)grid, threads, smem, st>>>(x, l);
     return launched();
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int WQ>
 static int launch_keys(const AttnArgs& x, LongArgs l, cudaStream_t st) {
-    constexpr int LD = tile_ld<T, DP>();
+    constexpr int LD = tile_ld<T, DP>(), threads = 128 * WQ;
     const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
-    const int smem = 6 * kTile * LD * (int)sizeof(T) + 4 * kTile * 16 + 2 * kTile * 8 + classes * 4 * (1 + kLongThreads);
+    const int smem = kTabBytes + 6 * kTile * LD * (int)sizeof(T) + 4 * kTile * 16 + 2 * kTile * 8 + classes * 4 * threads;
     l.tiles = (x.N + kTile - 1) / kTile;
     const int64_t grid = x.B * x.H * l.tiles;
     if (grid > 0x7fffffff) return HV_EINVAL;
     int n = 0;
-    int rc = resident_blocks(k_attn_keys<T, DP>, kLongThreads, smem, &n);
+    int rc = resident_blocks(k_attn_keys<T, DP, WQ>, threads, smem, &n);
     if (rc) return rc;
     if (grid) {
-        k_attn_keys<T, DP><<<(unsigned)grid, kLongThreads, smem, st>>>(x, l);
+        k_attn_keys<T, DP, WQ><<<(unsigned)grid, threads, smem, st>>>(x, l);
         if ((rc = launched())) return rc;
     }
     k_attn_table_sum<T><<<(classes * x.H + 7) / 8, 1024, 0, st>>>(x.partial, x.B * l.tiles, W, classes, x.H, x.dbq, x.dbr, x.dbz,
@@ -299,15 +293,23 @@ static int launch_keys(const AttnArgs& x, LongArgs l, cudaStream_t st) {
     return launched();
 }
 
+// 64 queries (keys) a block.  With too few such blocks to give every scheduler
+// several warps, two warps share each 16 of them; with too few for the SMs, or
+// few queries, a block takes 16 queries and four warps share them.
 template <typename T, bool BACK>
 static int launch_long(const AttnArgs& x, const LongArgs& l, cudaStream_t st) {
+    const int64_t heads = x.B * x.H, q_blocks = heads * ((x.Nq + kTile - 1) / kTile), k_blocks = heads * ((x.N + kTile - 1) / kTile);
+    const int sms = sm_count();
     auto go = [&](auto dim) -> int {
         constexpr int DP = decltype(dim)::value;
         int rc = HV_OK;
-        if (x.B && x.Nq)
-            rc = few_queries(x) ? launch_query<T, DP, 16, BACK>(x, l, st) : launch_query<T, DP, 64, BACK>(x, l, st);
+        if (q_blocks) {
+            if (x.Nq <= 16 || q_blocks < sms / 2) rc = launch_query<T, DP, 16, 4, BACK>(x, l, st);
+            else if (q_blocks < 4 * sms) rc = launch_query<T, DP, 64, 2, BACK>(x, l, st);
+            else rc = launch_query<T, DP, 64, 1, BACK>(x, l, st);
+        }
         if constexpr (BACK)
-            if (!rc) rc = launch_keys<T, DP>(x, l, st);
+            if (!rc) rc = k_blocks < 4 * sms ? launch_keys<T, DP, 2>(x, l, st) : launch_keys<T, DP, 1>(x, l, st);
         return rc;
     };
     switch (pad_dim(x.D)) {
@@ -494,7 +496,7 @@ int hv_relative_attention_forward(const hv_attention* a, void* out, void* saved,
     }
     LongArgs l = {};
     long_saved(a, saved ? saved : workspace, saved != nullptr, &l);
-    l.vec_in = vec_in(x, e, false);
+    l.vec_in = vec_in(x, e, false), l.vec_out = vec_out(x, e, false);
     if (x.B > 0x7fffffff) return HV_EINVAL;
     k_attn_sort<<<(unsigned)x.B, x.N <= 256 ? 256 : 1024, 0, st>>>(x, l);
     if (launched()) return HV_ECUDA;
@@ -530,7 +532,7 @@ int hv_relative_attention_backward(const hv_attention* a, const void* dout, cons
     LongArgs l = {};
     long_saved(a, const_cast<void*>(saved), true, &l);
     long_workspace(a, workspace, &l, &x.partial);
-    l.vec_in = vec_in(x, e, true);
+    l.vec_in = vec_in(x, e, true), l.vec_out = vec_out(x, e, true);
     return by_type(a->dtype, [&](auto t) { return launch_long<decltype(t), true>(x, l, st); });
 }
 
