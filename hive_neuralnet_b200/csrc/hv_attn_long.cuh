@@ -124,8 +124,10 @@ struct Classes {
     }
 };
 
-__device__ __forceinline__ float bias_of(const char* smem, const Classes& c) {
-    return *reinterpret_cast<const float*>(smem + (c.z * c.W + c.q)) + *reinterpret_cast<const float*>(smem + c.r + kTabR * 4);
+// The bias, in two terms.
+__device__ __forceinline__ float2 bias_of(const char* smem, const Classes& c) {
+    return make_float2(*reinterpret_cast<const float*>(smem + (c.z * c.W + c.q)),
+                       *reinterpret_cast<const float*>(smem + c.r + kTabR * 4));
 }
 
 // BACK false: the forward pass; true: dq (and delta).  A warp takes 16 of the
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
     using Op = Tile<T, DP == 8>;
     constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = ROWS * 2 * WK;
     constexpr int NT = 8 / WK;          // 8-key tiles of a warp
-    constexpr int NB = NT < 4 ? NT : 4;
+    constexpr int NB = NT < 4 ? NT : 4, CB = sizeof(T) == 4 && NC > 4 ? 4 : NC;
     // The output before rounding gives the backward pass its sum_j p dp, which it
     // takes from every dp: there the probabilities need all 24 bits.
     constexpr int PARTS = BACK || sizeof(T) == 4 ? kParts<T> : __is_same(T, __half) ? 2 : 3;
@@ -213,7 +215,8 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
             if (row < nq && t == 0 && part == 0) l.delta[head * l.Qpad + q0 + row] = delta[r];
         }
     }
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, acc[NC][4];
+    float top[2] = {-INFINITY, -INFINITY}, new_top[2], total[2], acc[NC][4];
+    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
     for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -235,26 +238,22 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
                 for (int e = 0; e < 4; e++) dp[j][e] = -delta[e >> 1];
 #pragma unroll
         for (int d = 0; d < DP; d += Op::KD) {
-            typename Op::A qa;
-            Op::load_a(qa, sq + row0 * LD + d, LD, lane);
+            typename Op::A qa[1];
+            Op::load_a(qa[0], sq + row0 * LD + d, LD, lane);
 #pragma unroll
             for (int j = 0; j < NT; j += NB) {
                 typename Op::B kb[NB];
                 Op::load_bn(kb, tk + j * 8 * LD + d, LD, lane);
-#pragma unroll
-                for (int x = 0; x < NB; x++) {
-                    if (d == 0) Op::template mma_d<true>(s[j + x], qa, kb[x]);
-                    else Op::mma_d(s[j + x], qa, kb[x]);
-                }
+                if (d == 0) Op::template product_d<true>(s + j, qa, kb);
+                else Op::template product_d<false>(s + j, qa, kb);
             }
             if constexpr (BACK) {
-                Op::load_a(qa, sg + row0 * LD + d, LD, lane);
+                Op::load_a(qa[0], sg + row0 * LD + d, LD, lane);
 #pragma unroll
                 for (int j = 0; j < NT; j += NB) {
                     typename Op::B vb[NB];
                     Op::load_bn(vb, tv + j * 8 * LD + d, LD, lane);
-#pragma unroll
-                    for (int x = 0; x < NB; x++) Op::mma_d(dp[j + x], qa, vb[x]);
+                    Op::template product_d<false>(dp + j, qa, vb);
                 }
             }
         }
@@ -262,10 +261,14 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
         for (int j = 0; j < NT; j++) {
             const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int r = e >> 1;
-                cls.of(e & 1 ? mb.x : ma.x, e & 1 ? mb.y : ma.y, e & 1 ? mb.z : ma.z, qq[r], qr[r], qz[r]);
-                s[j][e] = fmaf(s[j][e], scale2, bias_of(smem, cls));
+            for (int r = 0; r < 2; r++) {
+                cls.of(ma.x, ma.y, ma.z, qq[r], qr[r], qz[r]);
+                const float2 ba = bias_of(smem, cls);
+                cls.of(mb.x, mb.y, mb.z, qq[r], qr[r], qz[r]);
+                const float2 bb = bias_of(smem, cls);
+                const float2 x = fma2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(scale2, scale2),
+                                      add2(make_float2(ba.x, bb.x), make_float2(ba.y, bb.y)));
+                s[j][2 * r] = x.x, s[j][2 * r + 1] = x.y;
             }
         }
         if (left < NT * 8)  // the last tile
@@ -275,33 +278,51 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
                 for (int e = 0; e < 4; e++)
                     if (8 * j + 2 * t + (e & 1) >= left) s[j][e] = -INFINITY;
         if constexpr (!BACK) {
-            float base[2];
+            // The exponentials are taken against a reference that follows the row's
+            // maximum only when it is passed by more than 2^8: fp32 sums do not
+            // mind, and most tiles leave the accumulators alone.
+            bool passed = false;
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                float high = top[r];
+                float high = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < NT; j++) high = fmaxf(high, fmaxf(s[j][2 * r], s[j][2 * r + 1]));
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
-                base[r] = high == -INFINITY ? 0.f : high;  // no key of this warp's yet
-                const float f = exp2_approx(top[r] - base[r]);
-                top[r] = high;
-                sum[r] *= f;
+                passed = passed || high > top[r] + 8.f;
+                new_top[r] = high;
+            }
+            if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
-                for (int c = 0; c < NC; c++) acc[c][2 * r] *= f, acc[c][2 * r + 1] *= f;
+                for (int r = 0; r < 2; r++) {
+                    float high = fmaxf(new_top[r], top[r]);
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 1));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 2));
+                    const float f = high == -INFINITY ? 1.f : exp2_approx(top[r] - high);
+                    top[r] = high;
+                    sum[r].x *= f, sum[r].y *= f;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) acc[c][2 * r] *= f, acc[c][2 * r + 1] *= f;
+                }
             }
 #pragma unroll
-            for (int j = 0; j < NT; j++)
+            for (int r = 0; r < 2; r++) {
+                const float base = top[r] == -INFINITY ? 0.f : -top[r];  // no key of this warp's yet
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    s[j][e] = exp2_approx(s[j][e] - base[e >> 1]);
-                    sum[e >> 1] += s[j][e];
+                for (int j = 0; j < NT; j++) {
+                    float2 x = add2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(base, base));
+                    x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
+                    sum[r] = add2(sum[r], x);
+                    s[j][2 * r] = x.x, s[j][2 * r + 1] = x.y;
                 }
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < NT; j++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[j][e] = exp2_approx(s[j][e] - lse[e >> 1]) * dp[j][e];
+                for (int r = 0; r < 2; r++) {
+                    float2 x = add2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(-lse[r], -lse[r]));
+                    x = mul2(make_float2(exp2_approx(x.x), exp2_approx(x.y)), make_float2(dp[j][2 * r], dp[j][2 * r + 1]));
+                    s[j][2 * r] = x.x, s[j][2 * r + 1] = x.y;
+                }
         }
         const T* tb = BACK ? tk : tv;
 #pragma unroll
@@ -309,19 +330,19 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
             typename Op::A pa[PARTS];
             Op::a_from_c(pa, s + x / 8);
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                typename Op::B vb;
+            for (int c = 0; c < NC; c += CB) {
+                typename Op::B vb[CB];
                 Op::load_bk(vb, tb + x * LD + 8 * c, LD, lane);
-#pragma unroll
-                for (int y = 0; y < PARTS; y++) Op::mma(acc[c], pa[y], vb);
+                Op::template product<false>(acc + c, pa, vb);
             }
         }
     }
     cp_async_wait<0>();
 #pragma unroll
     for (int r = 0; r < 2; r++) {
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-        sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        total[r] = sum[r].x + sum[r].y;
+        total[r] += __shfl_xor_sync(0xffffffffu, total[r], 1);
+        total[r] += __shfl_xor_sync(0xffffffffu, total[r], 2);
     }
     if (WK > 1) {
         // join the key parts of a row, in their order, in the first part's warp
@@ -335,7 +356,7 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) mine[(g + 8 * r) * JL + 8 * c + 2 * t + e] = acc[c][2 * r + e];
-            if (t == 0) mine[(g + 8 * r) * JL + DP] = top[r], mine[(g + 8 * r) * JL + DP + 1] = sum[r];
+            if (t == 0) mine[(g + 8 * r) * JL + DP] = top[r], mine[(g + 8 * r) * JL + DP + 1] = total[r];
         }
         __syncthreads();
         if (part) return;
@@ -345,11 +366,11 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
             float high = -INFINITY, w[WK];
 #pragma unroll
             for (int x = 0; x < WK; x++) high = fmaxf(high, p[x * ROWS * JL + DP]);
-            sum[r] = 0.f;
+            total[r] = 0.f;
 #pragma unroll
             for (int x = 0; x < WK; x++) {
                 w[x] = BACK ? 1.f : exp2_approx(p[x * ROWS * JL + DP] - high);
-                sum[r] += w[x] * p[x * ROWS * JL + DP + 1];
+                total[r] += w[x] * p[x * ROWS * JL + DP + 1];
             }
             top[r] = high;
 #pragma unroll
@@ -368,8 +389,8 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
         const int row = row0 + g + 8 * r;
         if (row >= nq) continue;
         const int64_t at = head * l.Qpad + q0 + row;
-        if (!BACK && l.lse && t == 0) l.lse[at] = top[r] + log2f(sum[r]);
-        const float f = BACK ? a.scale : 1.f / sum[r];
+        if (!BACK && l.lse && t == 0) l.lse[at] = top[r] + log2f(total[r]);
+        const float f = BACK ? a.scale : 1.f / total[r];
         T* dst = out + qm[row].w * a.gs[1];
 #pragma unroll
         for (int c = 0; c < NC; c++) {
@@ -392,37 +413,37 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
     }
 }
 
-// dk, dv and the bias sums of 64 keys of one head.  A warp takes 16 of the keys
-// and, of each tile's queries, 32 at a time: all of them in turn, or (WQ = 2)
-// one half.
-template <typename T, int DP, int WQ>
-__global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const LongArgs l) {
+// dk, dv and the bias sums of KEYS keys of one head.  A warp takes 16 of the
+// keys and, of each tile's queries, 32 at a time: all of them in turn, or (WQ =
+// 2) one half.
+template <typename T, int DP, int KEYS, int WQ>
+__global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
-    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = 128 * WQ, PARTS = kParts<T>;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, CB = NC < 4 ? NC : 4, THREADS = 2 * KEYS * WQ, PARTS = kParts<T>;
     extern __shared__ __align__(16) char smem[];
     T* sk = reinterpret_cast<T*>(smem + kTabBytes);
-    T* sv = sk + kTile * LD;
-    T* sq = sv + kTile * LD;  // two stages of q, then of dout
+    T* sv = sk + KEYS * LD;
+    T* sq = sv + KEYS * LD;  // two stages of q, then of dout
     T* sg = sq + 2 * kTile * LD;
     int4* sm = reinterpret_cast<int4*>(sg + 2 * kTile * LD);  // three tiles of query meta
     int4* km = sm + 3 * kTile;                                // the keys' meta
-    float2* sd = reinterpret_cast<float2*>(km + kTile);       // two tiles of (lse, -delta)
+    float2* sd = reinterpret_cast<float2*>(km + KEYS);       // two tiles of (lse, -delta)
     float* hist = reinterpret_cast<float*>(sd + 2 * kTile);   // [warp][class][lane]
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int key0 = warp % 4 * 16, half = warp / 4;
+    const int key0 = warp % (KEYS / 16) * 16, half = warp / (KEYS / 16);
     const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
     const int64_t b = blockIdx.x / l.tiles / a.H;
     const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
     const int2 count = l.count[b];
-    const int k0 = tile * kTile, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below 64
+    const int k0 = tile * KEYS, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below KEYS
     const int4* meta = l.meta + b * l.Npad;
     const int64_t head = b * a.H + h;
     float* part = a.partial + ((b * l.tiles + tile) * classes) * a.H + h;
     T* dk = static_cast<T*>(a.dk) + b * a.gks[0] + h * a.gks[2];
     T* dv = static_cast<T*>(a.dv) + b * a.gks[0] + h * a.gks[2];
-    if (n < kTile)  // masked keys: zeros
-        for (int i = threadIdx.x; i < kTile * a.D; i += THREADS) {
+    if (n < KEYS)  // masked keys: zeros
+        for (int i = threadIdx.x; i < KEYS * a.D; i += THREADS) {
             const int r = i / a.D, d = i - r * a.D;
             if (r >= n && k0 + r < a.N) {
                 const int64_t at = meta[k0 + r].w * a.gks[1] + d;
@@ -435,10 +456,11 @@ __global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const 
     }
     const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
     const T* go = static_cast<const T*>(a.dout) + b * a.os[0] + h * a.os[2];
-    for (int i = threadIdx.x; i < kTile; i += THREADS) km[i] = meta[k0 + i], sm[i] = meta[i];
+    for (int i = threadIdx.x; i < KEYS; i += THREADS) km[i] = meta[k0 + i];
+    for (int i = threadIdx.x; i < kTile; i += THREADS) sm[i] = meta[i];
     __syncthreads();
-    load_tile<T, DP, kTile, THREADS>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
-    load_tile<T, DP, kTile, THREADS>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, KEYS, THREADS>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, KEYS, THREADS>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
     const int tiles = (nq + kTile - 1) / kTile;
     auto issue = [&](int i) {
         if (i < tiles) {
@@ -461,7 +483,7 @@ __global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const 
     load_bias_table<T>(smem, a, h);
     for (int i = threadIdx.x; i < classes * THREADS; i += THREADS) hist[i] = 0.f;
     const float scale2 = a.scale * kLog2E;
-    char* sums = reinterpret_cast<char*>(hist + warp * classes * 32 + lane);
+    const uint32_t hq = smem_addr(hist + warp * classes * 32 + lane), hr = hq + W * 128, hz = hr + W * 128;
     Classes cls(a);
     int kq[2], kr[2], kz[2];
     bool live[2];
@@ -496,38 +518,35 @@ __global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const 
             }
 #pragma unroll
             for (int d = 0; d < DP; d += Op::KD) {
-                typename Op::A ka;
+                typename Op::A ka[1];
                 typename Op::B qb[4];
-                Op::load_a(ka, sk + key0 * LD + d, LD, lane);
+                Op::load_a(ka[0], sk + key0 * LD + d, LD, lane);
                 Op::load_bn(qb, tq + d, LD, lane);
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    if (d == 0) Op::template mma_d<true>(s[x], ka, qb[x]);
-                    else Op::mma_d(s[x], ka, qb[x]);
-                }
-                Op::load_a(ka, sv + key0 * LD + d, LD, lane);
+                if (d == 0) Op::template product_d<true>(s, ka, qb);
+                else Op::template product_d<false>(s, ka, qb);
+                Op::load_a(ka[0], sv + key0 * LD + d, LD, lane);
                 Op::load_bn(qb, tg + d, LD, lane);
-#pragma unroll
-                for (int x = 0; x < 4; x++) Op::mma_d(dp[x], ka, qb[x]);
+                Op::template product_d<false>(dp, ka, qb);
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
                 const float4 x = *reinterpret_cast<const float4*>(td + 8 * j + 2 * t);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int r = e >> 1;
-                    cls.of(kq[r], kr[r], kz[r], -(e & 1 ? mb.x : ma.x), -(e & 1 ? mb.y : ma.y), -(e & 1 ? mb.z : ma.z));
-                    const float y2 = fmaf(s[j][e], scale2, bias_of(smem, cls));
-                    s[j][e] = live[r] ? exp2_approx(y2 - (e & 1 ? x.z : x.x)) : 0.f;
-                    dp[j][e] *= s[j][e];
-                    float* hq = reinterpret_cast<float*>(sums + cls.q * 32);
-                    float* hr = reinterpret_cast<float*>(sums + W * 128 + cls.r * 32);
-                    float* hz = reinterpret_cast<float*>(sums + 2 * W * 128 + cls.z * 32);
-                    const float xq = *hq, xr = *hr, xz = *hz;
-                    *hq = xq + dp[j][e];
-                    *hr = xr + dp[j][e];
-                    *hz = xz + dp[j][e];
+                for (int r = 0; r < 2; r++) {
+                    Classes ca = cls, cb = cls;
+                    ca.of(kq[r], kr[r], kz[r], -ma.x, -ma.y, -ma.z);
+                    cb.of(kq[r], kr[r], kz[r], -mb.x, -mb.y, -mb.z);
+                    const float2 ba = bias_of(smem, ca), bb = bias_of(smem, cb);
+                    float2 y2 = fma2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(scale2, scale2),
+                                     add2(make_float2(ba.x, bb.x), make_float2(ba.y, bb.y)));
+                    y2 = add2(y2, make_float2(-x.x, -x.z));
+                    s[j][2 * r] = live[r] ? exp2_approx(y2.x) : 0.f;
+                    s[j][2 * r + 1] = live[r] ? exp2_approx(y2.y) : 0.f;
+                    const float2 ds = mul2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(dp[j][2 * r], dp[j][2 * r + 1]));
+                    dp[j][2 * r] = ds.x, dp[j][2 * r + 1] = ds.y;
+                    add_at(hq + ca.q * 32, hr + ca.r * 32, hz + ca.z * 32, ds.x);
+                    add_at(hq + cb.q * 32, hr + cb.r * 32, hz + cb.z * 32, ds.y);
                 }
             }
 #pragma unroll
@@ -535,19 +554,17 @@ __global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const 
                 typename Op::A pa[PARTS];
                 Op::a_from_c(pa, s + x / 8);
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    typename Op::B gb;
+                for (int c = 0; c < NC; c += CB) {
+                    typename Op::B gb[CB];
                     Op::load_bk(gb, tg + x * LD + 8 * c, LD, lane);
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++) Op::mma(av[c], pa[p], gb);
+                    Op::template product<false>(av + c, pa, gb);
                 }
                 Op::a_from_c(pa, dp + x / 8);
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    typename Op::B qb;
+                for (int c = 0; c < NC; c += CB) {
+                    typename Op::B qb[CB];
                     Op::load_bk(qb, tq + x * LD + 8 * c, LD, lane);
-#pragma unroll
-                    for (int p = 0; p < PARTS; p++) Op::mma(ak[c], pa[p], qb);
+                    Op::template product<false>(ak + c, pa, qb);
                 }
             }
         }
@@ -604,7 +621,7 @@ __global__ void __launch_bounds__(128 * WQ) k_attn_keys(const AttnArgs a, const 
     __syncthreads();
     for (int c = threadIdx.x; c < classes; c += THREADS) {
         float x = 0.f;
-        for (int w = 0; w < 4 * WQ; w++) x += hist[(w * classes + c) * 32];
+        for (int w = 0; w < KEYS / 16 * WQ; w++) x += hist[(w * classes + c) * 32];
         part[(int64_t)c * a.H] = x;
     }
 }

@@ -107,7 +107,7 @@ struct ClassOf {
 template <typename T, int DP, bool BACK>
 __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const ShortPlan p) {
     using Op = Tile<T, DP == 8>;
-    constexpr int NC = DP / 8, PARTS = kParts<T>;  // 8-value chunks of a head
+    constexpr int NC = DP / 8, CB = NC < 4 ? NC : 4, PARTS = kParts<T>;  // 8-value chunks of a head
     constexpr bool F32 = sizeof(T) == 4;
     extern __shared__ __align__(16) char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
             const char* bias = reinterpret_cast<const char*>(tab + warp * classes);
             const char* bias_r = bias + W * 4;
             const char* bias_z = bias + 2 * W * 4;
-            char* sums = reinterpret_cast<char*>(hist + warp * classes * 32 + lane);
+            const uint32_t hq = smem_addr(hist + warp * classes * 32 + lane), hr = hq + W * 128, hz = hr + W * 128;
             float dk[2][NC][4], dv[2][NC][4];
             if (BACK)
 #pragma unroll
@@ -220,19 +220,23 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                     for (int e = 0; e < 4; e++) s[i][e] = dp[i][e] = 0.f;
 #pragma unroll
                 for (int d = 0; d < DP; d += Op::KD) {
-                    typename Op::A qa;
-                    typename Op::B kb[4];
-                    Op::load_a(qa, Q + m0 * ld + d, ld, lane);
+                    typename Op::A qa[1];
+                    typename Op::B kb[2];
+                    Op::load_a(qa[0], Q + m0 * ld + d, ld, lane);
                     Op::load_bn(kb, K + d, ld, lane);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (8 * i < n) Op::mma_d(s[i], qa, kb[i]);
+                    Op::template product_d<false>(s, qa, kb);
+                    if (n > 16) {
+                        Op::load_bn(kb, K + 16 * ld + d, ld, lane);
+                        Op::template product_d<false>(s + 2, qa, kb);
+                    }
                     if (BACK) {
-                        Op::load_a(qa, G + m0 * ld + d, ld, lane);
+                        Op::load_a(qa[0], G + m0 * ld + d, ld, lane);
                         Op::load_bn(kb, V + d, ld, lane);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (8 * i < n) Op::mma_d(dp[i], qa, kb[i]);
+                        Op::template product_d<false>(dp, qa, kb);
+                        if (n > 16) {
+                            Op::load_bn(kb, V + 16 * ld + d, ld, lane);
+                            Op::template product_d<false>(dp + 2, qa, kb);
+                        }
                     }
                 }
                 int q4[2][3];
@@ -295,11 +299,10 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                         typename Op::A pa[PARTS];
                         Op::a_from_c(pa, s + k / 8);
 #pragma unroll
-                        for (int c = 0; c < NC; c++) {
-                            typename Op::B vb;
+                        for (int c = 0; c < NC; c += CB) {
+                            typename Op::B vb[CB];
                             Op::load_bk(vb, V + k * ld + 8 * c, ld, lane);
-#pragma unroll
-                            for (int x = 0; x < PARTS; x++) Op::mma(o[c], pa[x], vb);
+                            Op::template product<false>(o + c, pa, vb);
                         }
                     }
                     __syncwarp();
@@ -336,60 +339,55 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int r = e >> 1;
-                            float* hq = reinterpret_cast<float*>(sums + cls.q(e & 1 ? kq.y : kq.x, q4[r][0]) * 32);
-                            float* hr = reinterpret_cast<float*>(sums + W * 128 + cls.q(e & 1 ? kr.y : kr.x, q4[r][1]) * 32);
-                            float* hz = reinterpret_cast<float*>(sums + 2 * W * 128 + cls.z(e & 1 ? kz.y : kz.x, q4[r][2]) * 32);
-                            const float xq = *hq, xr = *hr, xz = *hz;
-                            *hq = xq + dp[i][e];
-                            *hr = xr + dp[i][e];
-                            *hz = xz + dp[i][e];
+                            add_at(hq + cls.q(e & 1 ? kq.y : kq.x, q4[r][0]) * 32, hr + cls.q(e & 1 ? kr.y : kr.x, q4[r][1]) * 32,
+                                   hz + cls.z(e & 1 ? kz.y : kz.x, q4[r][2]) * 32, dp[i][e]);
                         }
                     }
-                    typename Op::A pt[PARTS][2][16 / Op::KK];
+                    typename Op::A pt[2][16 / Op::KK][PARTS];
                     float* room = scratch + (F32 ? warp * 16 * kTransposeLd : 0);
                     transpose_c<T, DP == 8>(pt, s, room, lane);
 #pragma unroll
                     for (int k = 0; k < 16 / Op::KK; k++)
 #pragma unroll
-                        for (int c = 0; c < NC; c++) {
-                            typename Op::B gb;
+                        for (int c = 0; c < NC; c += CB) {
+                            typename Op::B gb[CB];
                             Op::load_bk(gb, G + (m0 + k * Op::KK) * ld + 8 * c, ld, lane);
-#pragma unroll
-                            for (int y = 0; y < PARTS; y++) {
-                                Op::mma(dv[0][c], pt[y][0][k], gb);
-                                if (n > 16) Op::mma(dv[1][c], pt[y][1][k], gb);
-                            }
+                            Op::template product<false>(dv[0] + c, pt[0][k], gb);
+                            if (n > 16) Op::template product<false>(dv[1] + c, pt[1][k], gb);
                         }
                     transpose_c<T, DP == 8>(pt, dp, room, lane);
 #pragma unroll
                     for (int k = 0; k < 16 / Op::KK; k++)
 #pragma unroll
-                        for (int c = 0; c < NC; c++) {
-                            typename Op::B qb;
+                        for (int c = 0; c < NC; c += CB) {
+                            typename Op::B qb[CB];
                             Op::load_bk(qb, Q + (m0 + k * Op::KK) * ld + 8 * c, ld, lane);
-#pragma unroll
-                            for (int y = 0; y < PARTS; y++) {
-                                Op::mma(dk[0][c], pt[y][0][k], qb);
-                                if (n > 16) Op::mma(dk[1][c], pt[y][1][k], qb);
-                            }
+                            Op::template product<false>(dk[0] + c, pt[0][k], qb);
+                            if (n > 16) Op::template product<false>(dk[1] + c, pt[1][k], qb);
                         }
                     __syncwarp();  // this tile's rows of Q are done with: dq takes their place
 #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        float o[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int c = 0; c < NC; c += CB) {
+                        float o[CB][4];
+#pragma unroll
+                        for (int z = 0; z < CB; z++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[z][e] = 0.f;
 #pragma unroll
                         for (int k = 0; k < kSlots; k += Op::KK) {
                             if (k >= n) continue;
                             typename Op::A da[PARTS];
-                            typename Op::B kb;
+                            typename Op::B kb[CB];
                             Op::a_from_c(da, dp + k / 8);
                             Op::load_bk(kb, K + k * ld + 8 * c, ld, lane);
-#pragma unroll
-                            for (int y = 0; y < PARTS; y++) Op::mma(o, da[y], kb);
+                            Op::template product<false>(o, da, kb);
                         }
-                        float lo[2] = {o[0] * a.scale, o[1] * a.scale}, hi[2] = {o[2] * a.scale, o[3] * a.scale};
-                        store_vec<T, 2>(Q + (m0 + g) * ld + 8 * c + 2 * t, lo);
-                        store_vec<T, 2>(Q + (m0 + g + 8) * ld + 8 * c + 2 * t, hi);
+#pragma unroll
+                        for (int z = 0; z < CB; z++) {
+                            float lo[2] = {o[z][0] * a.scale, o[z][1] * a.scale}, hi[2] = {o[z][2] * a.scale, o[z][3] * a.scale};
+                            store_vec<T, 2>(Q + (m0 + g) * ld + 8 * (c + z) + 2 * t, lo);
+                            store_vec<T, 2>(Q + (m0 + g + 8) * ld + 8 * (c + z) + 2 * t, hi);
+                        }
                     }
                 }
             }

@@ -59,6 +59,27 @@ __device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 
+// A pair of fp32 values in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 c;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{ .reg .b64 w, x, y, z; mov.b64 w, {%2, %3}; mov.b64 x, {%4, %5}; mov.b64 y, {%6, %7}; fma.rn.f32x2 z, w, x, y; "
+        "mov.b64 {%0, %1}, z; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
 // c = a b + (FIRST ? 0 : c)
 #define HV_MMA(NAME, SHAPE, TYPES, NA, AREGS, BREGS)                                                                    \
     template <bool FIRST>                                                                                               \
@@ -99,45 +120,74 @@ struct Tile {  // 16-bit types
     struct A { uint32_t r[4]; };
     struct B { uint32_t r[2]; };
 
-    template <bool FIRST = false>
-    __device__ static void mma(float* c, const A& a, const B& b) {
-        if constexpr (__is_same(T, __half)) mma_f16_k16<FIRST>(c, a.r, b.r);
-        else mma_bf16_k16<FIRST>(c, a.r, b.r);
+    // c[i] = (FIRST ? 0 : c[i]) + the parts of a times b[i], a step along tokens.
+    // One part for all tiles, then the next: a tile's products are far apart.
+    template <bool FIRST, int PARTS, int N>
+    __device__ static void product(float (*c)[4], const A (&a)[PARTS], const B (&b)[N]) {
+#pragma unroll
+        for (int p = 0; p < PARTS; p++)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if constexpr (__is_same(T, __half)) {
+                    if (p == 0) mma_f16_k16<FIRST>(c[i], a[p].r, b[i].r);
+                    else mma_f16_k16<false>(c[i], a[p].r, b[i].r);
+                } else {
+                    if (p == 0) mma_bf16_k16<FIRST>(c[i], a[p].r, b[i].r);
+                    else mma_bf16_k16<false>(c[i], a[p].r, b[i].r);
+                }
+            }
     }
-    template <bool FIRST = false>
-    __device__ static void mma_d(float* c, const A& a, const B& b) {
-        if constexpr (!D8) mma<FIRST>(c, a, b);
-        else if constexpr (__is_same(T, __half)) mma_f16_k8<FIRST>(c, a.r, b.r);
-        else mma_bf16_k8<FIRST>(c, a.r, b.r);
+    // ... a step along the head's values
+    template <bool FIRST, int N>
+    __device__ static void product_d(float (*c)[4], const A (&a)[1], const B (&b)[N]) {
+        if constexpr (!D8) {
+            product<FIRST>(c, a, b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if constexpr (__is_same(T, __half)) mma_f16_k8<FIRST>(c[i], a[0].r, b[i].r);
+                else mma_bf16_k8<FIRST>(c[i], a[0].r, b[i].r);
+            }
+        }
     }
     // 16 rows x KD values at p (row-major, ld elements a row)
     __device__ static void load_a(A& a, const T* p, int ld, int lane) {
         if constexpr (D8) ldsm2(a.r[0], a.r[1], p + (lane & 15) * ld);
         else ldsm4(a.r, p + (lane & 15) * ld + (lane >> 4) * 8);
     }
-    // 16 or 32 rows x KD values at p as B operands (n = row)
-    __device__ static void load_bn(B (&b)[2], const T* p, int ld, int lane) {
-        if constexpr (D8) {
+    // NB * 8 rows x KD values at p as B operands (n = row)
+    template <int NB>
+    __device__ static void load_bn(B (&b)[NB], const T* p, int ld, int lane) {
+        uint32_t r[4];
+        if constexpr (!D8) {  // both halves of two operands at once: an operand's registers stay neighbours
+            const T* q = p + ((lane & 7) + (lane >> 4) * 8) * ld + (lane & 8);
+#pragma unroll
+            for (int n = 0; n < NB; n += 2) {
+                ldsm4(r, q + n * 8 * ld);
+                b[n].r[0] = r[0], b[n].r[1] = r[1], b[n + 1].r[0] = r[2], b[n + 1].r[1] = r[3];
+            }
+        } else if constexpr (NB == 2) {
             ldsm2(b[0].r[0], b[1].r[0], p + (lane & 15) * ld);
         } else {
+            ldsm4(r, p + lane * ld);
+#pragma unroll
+            for (int n = 0; n < 4; n++) b[n].r[0] = r[n];
+        }
+    }
+    // KK rows x 8 NB values at p as B operands (k = row)
+    template <int NB>
+    __device__ static void load_bk(B (&b)[NB], const T* p, int ld, int lane) {
+        if constexpr (NB == 1) {
+            ldsm2_t(b[0].r[0], b[0].r[1], p + (lane & 15) * ld);
+        } else {
             uint32_t r[4];
-            ldsm4(r, p + (lane & 15) * ld + (lane >> 4) * 8);
-            b[0].r[0] = r[0], b[1].r[0] = r[1], b[0].r[1] = r[2], b[1].r[1] = r[3];
+#pragma unroll
+            for (int n = 0; n < NB; n += 2) {
+                ldsm4_t(r, p + (lane & 15) * ld + (lane >> 4) * 8 + n * 8);
+                b[n].r[0] = r[0], b[n].r[1] = r[1], b[n + 1].r[0] = r[2], b[n + 1].r[1] = r[3];
+            }
         }
     }
-    __device__ static void load_bn(B (&b)[4], const T* p, int ld, int lane) {
-        uint32_t r[4];
-        ldsm4(r, p + lane * ld);
-#pragma unroll
-        for (int n = 0; n < 4; n++) b[n].r[0] = r[n];
-        if constexpr (!D8) {
-            ldsm4(r, p + lane * ld + 8);
-#pragma unroll
-            for (int n = 0; n < 4; n++) b[n].r[1] = r[n];
-        }
-    }
-    // KK rows x 8 values at p as a B operand (k = row)
-    __device__ static void load_bk(B& b, const T* p, int ld, int lane) { ldsm2_t(b.r[0], b.r[1], p + (lane & 15) * ld); }
     // C tiles of 16 rows x KK columns as PARTS A operands (k = column): the
     // values rounded, then what the rounding left, rounded, ...
     template <int PARTS>
@@ -149,8 +199,8 @@ struct Tile {  // 16-bit types
             for (int p = 0; p < PARTS; p++) {
                 a[p].r[i] = pack2(x, y, T());
                 if (p + 1 < PARTS) {
-                    const float2 f = unpack2(a[p].r[i], T());
-                    x -= f.x, y -= f.y;
+                    const float2 f = unpack2(a[p].r[i], T()), z = add2(make_float2(x, y), make_float2(-f.x, -f.y));
+                    x = z.x, y = z.y;
                 }
             }
         }
@@ -163,14 +213,17 @@ struct Tile<float, D8> {
     struct A { uint32_t hi[4], lo[4]; };
     struct B { uint32_t hi[2], lo[2]; };
 
-    template <bool FIRST = false>
-    __device__ static void mma(float* c, const A& a, const B& b) {
-        mma_tf32<FIRST>(c, a.lo, b.hi);
-        mma_tf32<false>(c, a.hi, b.lo);
-        mma_tf32<false>(c, a.hi, b.hi);
+    template <bool FIRST, int N>
+    __device__ static void product(float (*c)[4], const A (&a)[1], const B (&b)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; i++) mma_tf32<FIRST>(c[i], a[0].lo, b[i].hi);
+#pragma unroll
+        for (int i = 0; i < N; i++) mma_tf32<false>(c[i], a[0].hi, b[i].lo);
+#pragma unroll
+        for (int i = 0; i < N; i++) mma_tf32<false>(c[i], a[0].hi, b[i].hi);
     }
-    template <bool FIRST = false>
-    __device__ static void mma_d(float* c, const A& a, const B& b) { mma<FIRST>(c, a, b); }
+    template <bool FIRST, int N>
+    __device__ static void product_d(float (*c)[4], const A (&a)[1], const B (&b)[N]) { product<FIRST>(c, a, b); }
     __device__ static void load_a(A& a, const float* p, int ld, int lane) {
         const float* q = p + (lane >> 2) * ld + 2 * (lane & 3);
         const float2 x = *reinterpret_cast<const float2*>(q), y = *reinterpret_cast<const float2*>(q + 8 * ld);
@@ -188,10 +241,14 @@ struct Tile<float, D8> {
             split_tf32(x.y, b[n].hi[1], b[n].lo[1]);
         }
     }
-    __device__ static void load_bk(B& b, const float* p, int ld, int lane) {
+    template <int NB>
+    __device__ static void load_bk(B (&b)[NB], const float* p, int ld, int lane) {
         const float* q = p + 2 * (lane & 3) * ld + (lane >> 2);
-        split_tf32(q[0], b.hi[0], b.lo[0]);
-        split_tf32(q[ld], b.hi[1], b.lo[1]);
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            split_tf32(q[8 * n], b[n].hi[0], b[n].lo[0]);
+            split_tf32(q[ld + 8 * n], b[n].hi[1], b[n].lo[1]);
+        }
     }
     __device__ static void a_from_c(A (&a)[1], const float (*c)[4]) {
         split_tf32(c[0][0], a[0].hi[0], a[0].lo[0]);
@@ -209,12 +266,12 @@ template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 1 : 2;
 
 // The transpose of 16 x 32 C tiles (rows: queries, columns: keys) as A operands
-// [part][2][16 / KK] (m = key, k = query): in registers for 16-bit types,
+// [2][16 / KK][part] (m = key, k = query): in registers for 16-bit types,
 // through 16 x kTransposeLd floats of the warp's own for fp32.
 constexpr int kTransposeLd = 36;
 
 template <typename T, bool D8>
-__device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[kParts<T>][2][16 / Tile<T, D8>::KK],
+__device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[2][16 / Tile<T, D8>::KK][kParts<T>],
                                             const float (&c)[4][4], float* scratch, int lane) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -224,8 +281,8 @@ __device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[kParts<
                 const float* v = c[2 * m + (i & 1)] + 2 * (i >> 1);
                 const uint32_t first = pack2(v[0], v[1], T());
                 const float2 f = unpack2(first, T());
-                a[0][m][0].r[i] = transpose8(first);
-                a[1][m][0].r[i] = transpose8(pack2(v[0] - f.x, v[1] - f.y, T()));
+                a[m][0][0].r[i] = transpose8(first);
+                a[m][0][1].r[i] = transpose8(pack2(v[0] - f.x, v[1] - f.y, T()));
             }
     } else {
         const int g = lane >> 2, t = lane & 3;
@@ -241,7 +298,7 @@ __device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[kParts<
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const float* p = scratch + (8 * k + 2 * t) * kTransposeLd + 16 * m + g;
-                auto& x = a[0][m][k];
+                auto& x = a[m][k][0];
                 split_tf32(p[0], x.hi[0], x.lo[0]);
                 split_tf32(p[8], x.hi[1], x.lo[1]);
                 split_tf32(p[kTransposeLd], x.hi[2], x.lo[2]);
@@ -265,6 +322,20 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The bias sums' own accesses to shared memory.  Nothing else touches their
+// region while they run, so they carry no memory clobber: the loads of the next
+// values' tables may move ahead of them.
+__device__ __forceinline__ void add_at(uint32_t p, uint32_t q, uint32_t r, float x) {
+    float a, b, c;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(p));
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(b) : "r"(q));
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(c) : "r"(r));
+    a += x, b += x, c += x;
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(p), "f"(a));
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(q), "f"(b));
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(r), "f"(c));
 }
 
 __device__ __forceinline__ float rcp_approx(float x) {

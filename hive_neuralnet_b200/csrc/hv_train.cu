@@ -227,6 +227,8 @@ static bool vec_out(const AttnArgs& x, int e, bool back) {
 }
 
 // ---- any number of tokens
+constexpr int kKeysLeast = 32;  // keys a block, at least
+
 static int round_up(int x, int n) { return (x + n - 1) / n * n; }
 
 // What the forward pass leaves for the backward pass (or, without one, its
@@ -253,7 +255,7 @@ static size_t long_saved(const hv_attention* a, void* base, bool all, LongArgs* 
 
 static size_t long_workspace(const hv_attention* a, void* base, LongArgs* l, float** partial) {
     const size_t delta = round256((size_t)a->batch * a->heads * round_up(a->queries, kTile) * 4);
-    const int64_t blocks = a->batch * (round_up(a->tokens, kTile) / kTile);
+    const int64_t blocks = a->batch * (round_up(a->tokens, kTile) / kKeysLeast);
     l->delta = static_cast<float*>(base);
     *partial = base ? reinterpret_cast<float*>(static_cast<char*>(base) + delta) : nullptr;
     return delta + (size_t)blocks * attn_classes(a) * a->heads * 4;
@@ -273,19 +275,20 @@ static int launch_query(const AttnArgs& x, LongArgs l, cudaStream_t st) {
     return launched();
 }
 
-template <typename T, int DP, int WQ>
+template <typename T, int DP, int KEYS, int WQ>
 static int launch_keys(const AttnArgs& x, LongArgs l, cudaStream_t st) {
-    constexpr int LD = tile_ld<T, DP>(), threads = 128 * WQ;
+    constexpr int LD = tile_ld<T, DP>(), threads = 2 * KEYS * WQ;
     const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
-    const int smem = kTabBytes + 6 * kTile * LD * (int)sizeof(T) + 4 * kTile * 16 + 2 * kTile * 8 + classes * 4 * threads;
-    l.tiles = (x.N + kTile - 1) / kTile;
+    const int smem =
+        kTabBytes + (2 * KEYS + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + KEYS) * 16 + 2 * kTile * 8 + classes * 4 * threads;
+    l.tiles = (x.N + KEYS - 1) / KEYS;
     const int64_t grid = x.B * x.H * l.tiles;
     if (grid > 0x7fffffff) return HV_EINVAL;
     int n = 0;
-    int rc = resident_blocks(k_attn_keys<T, DP, WQ>, threads, smem, &n);
+    int rc = resident_blocks(k_attn_keys<T, DP, KEYS, WQ>, threads, smem, &n);
     if (rc) return rc;
     if (grid) {
-        k_attn_keys<T, DP, WQ><<<(unsigned)grid, threads, smem, st>>>(x, l);
+        k_attn_keys<T, DP, KEYS, WQ><<<(unsigned)grid, threads, smem, st>>>(x, l);
         if ((rc = launched())) return rc;
     }
     k_attn_table_sum<T><<<(classes * x.H + 7) / 8, 1024, 0, st>>>(x.partial, x.B * l.tiles, W, classes, x.H, x.dbq, x.dbr, x.dbz,
@@ -305,11 +308,11 @@ static int launch_long(const AttnArgs& x, const LongArgs& l, cudaStream_t st) {
         int rc = HV_OK;
         if (q_blocks) {
             if (x.Nq <= 16 || q_blocks < sms / 2) rc = launch_query<T, DP, 16, 4, BACK>(x, l, st);
-            else if (q_blocks < 4 * sms) rc = launch_query<T, DP, 64, 2, BACK>(x, l, st);
+            else if (q_blocks < 4 * sms) rc = launch_query<T, DP, 32, 2, BACK>(x, l, st);
             else rc = launch_query<T, DP, 64, 1, BACK>(x, l, st);
         }
         if constexpr (BACK)
-            if (!rc) rc = k_blocks < 4 * sms ? launch_keys<T, DP, 2>(x, l, st) : launch_keys<T, DP, 1>(x, l, st);
+            if (!rc) rc = k_blocks < 4 * sms ? launch_keys<T, DP, 32, 2>(x, l, st) : launch_keys<T, DP, 64, 1>(x, l, st);
         return rc;
     };
     switch (pad_dim(x.D)) {
