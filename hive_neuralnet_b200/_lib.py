@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -67,8 +68,20 @@ class HvAttention(C.Structure):
                 ("table_dtype", C.c_int32), ("scale", C.c_float)]
 
 
+# The same fields as bytes, in one call (filling a ctypes struct field by field takes several microseconds).
+pack_attention = struct.Struct("@3P9q4P4q3Pq8if4x").pack
+
+
+class _AttentionArg:
+    """const hv_attention*: a HvAttention, or pack_attention's bytes."""
+
+    @classmethod
+    def from_param(cls, arg):
+        return C.c_char_p.from_param(arg) if type(arg) is bytes else C.byref(arg)
+
+
 _tp = C.POINTER(HvTree)
-_ap = C.POINTER(HvAttention)
+_ap = _AttentionArg
 _f = C.c_float
 _sz = C.c_size_t
 

@@ -26,8 +26,8 @@ struct NormArgs {
     void *s, *y;                // forward outputs; s NULL without a residual
     float *mean, *rstd;
     const void *dy, *ds;  // backward
-    void* dx;
-    float* partial;  // [grid][2][C]
+    void *dx, *dw, *db;
+    float* partial;  // [grid][2][C]; not used by a single block
     int64_t rows;
     int C, G, w_f32;
     float eps;
@@ -179,7 +179,14 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
     }
     // this block's sums over its rows, in a fixed order: over the groups of a
     // warp by shuffles, over the warps through shared memory
+    // (a single block's are the results)
     float* out = a.partial + (int64_t)blockIdx.x * 2 * a.C;
+    auto put = [&](int which, int c, float x) {
+        if (gridDim.x == 1)
+            store_param<T>(which ? a.db : a.dw, c, a.w_f32, x);
+        else
+            out[which * a.C + c] = x;
+    };
     const int span = G < 32 ? G : 32, warp = threadIdx.x >> 5, l = threadIdx.x & 31;
 #pragma unroll
     for (int which = 0; which < 2; which++)
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
                 const int c = (k * G + lane) * V;
 #pragma unroll
                 for (int i = 0; i < V; i++)
-                    if (c + i < a.C) out[which * a.C + c + i] = v[i];
+                    if (c + i < a.C) put(which, c + i, v[i]);
                 continue;
             }
             __syncthreads();
@@ -207,7 +214,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
                 float t = 0.f;
                 for (int q = 0; q < (int)(blockDim.x >> 5); q++) t += part[q * G * V + j];
                 const int c = k * G * V + j;
-                if (c < a.C) out[which * a.C + c] = t;
+                if (c < a.C) put(which, c, t);
             }
         }
 }

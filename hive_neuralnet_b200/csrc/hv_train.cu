@@ -106,7 +106,10 @@ static int launch_norm(const NormArgs& a, const NormShape& s, int grid, cudaStre
     return HV_EINVAL;
 }
 
-static int norm_grid(const NormShape& s, int64_t rows) {
+// Backward: up to four turns of one block cost less than a second launch that
+// joins several blocks' sums.
+static int norm_grid(const NormShape& s, int64_t rows, bool back) {
+    if (back && rows <= 4 * (s.threads / s.G)) return 1;
     const int64_t blocks = (rows + s.threads / s.G - 1) / (s.threads / s.G), cap = (int64_t)sm_count() * kNormBlocksPerSm;
     return (int)(blocks < cap ? blocks : cap);
 }
@@ -354,7 +357,7 @@ int hv_layer_norm_forward(const void* x, const void* residual, const void* weigh
     NormArgs a = {};
     a.x = x, a.r = residual, a.w = weight, a.b = bias, a.s = sum, a.y = y, a.mean = mean, a.rstd = rstd;
     a.rows = rows, a.C = width, a.G = s.G, a.w_f32 = weight_dtype == HV_F32, a.eps = eps;
-    const int grid = norm_grid(s, rows);
+    const int grid = norm_grid(s, rows, false);
     return by_type(dtype, [&](auto t) { return launch_norm<decltype(t), false>(a, s, grid, (cudaStream_t)stream); });
 }
 
@@ -362,7 +365,9 @@ int hv_layer_norm_workspace_bytes(int64_t rows, int width, int dtype, size_t* by
     NormShape s, t;
     if (!bytes || rows < 0 || width < 1 || width > kNormMaxWidth || dtype < 0 || dtype > 2) return HV_EINVAL;
     if (!norm_shape(width, dtype, false, &s) || !norm_shape(width, dtype, true, &t)) return HV_EINVAL;
-    *bytes = (size_t)sm_count() * kNormBlocksPerSm * 2 * width * 4;
+    const int g = norm_grid(s, rows, true), h = norm_grid(t, rows, true);
+    *bytes = (size_t)(g > h ? g : h) * 2 * width * 4;
+    if (*bytes < 16) *bytes = 16;
     return HV_OK;
 }
 
@@ -375,18 +380,18 @@ int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     if (rows && (!dy || !x || !weight || !mean || !rstd || !dx)) return HV_EINVAL;
     NormShape s;
     if (!norm_shape(width, dtype, norm_vec(width, dtype, {dy, x, dsum, dx}), &s)) return HV_EINVAL;
-    const int grid = rows ? norm_grid(s, rows) : 0;
+    const int grid = rows ? norm_grid(s, rows, true) : 0;
     if (workspace_bytes < (size_t)grid * 2 * width * 4) return HV_EINVAL;
     NormArgs a = {};
     a.x = x, a.w = weight, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
-    a.dy = dy, a.ds = dsum, a.dx = dx, a.partial = static_cast<float*>(workspace);
+    a.dy = dy, a.ds = dsum, a.dx = dx, a.dw = dweight, a.db = dbias, a.partial = static_cast<float*>(workspace);
     a.rows = rows, a.C = width, a.G = s.G, a.w_f32 = weight_dtype == HV_F32;
     const cudaStream_t st = (cudaStream_t)stream;
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (grid) {
             const int rc = launch_norm<T, true>(a, s, grid, st);
-            if (rc) return rc;
+            if (rc || grid == 1) return rc;
         }
         k_norm_reduce<T><<<(2 * width + 31) / 32, 1024, 0, st>>>(a.partial, grid, width, dweight, dbias, a.w_f32);
         return launched();

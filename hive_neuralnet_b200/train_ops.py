@@ -18,6 +18,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
+from operator import attrgetter
 
 import torch
 
@@ -28,6 +30,11 @@ MAX_HEAD_DIM = 64
 MAX_COORD_CLIP, MAX_HEIGHT_CLIP = 16, 4
 MAX_NORM_WIDTH = 8192
 STATE_BLOCK = 256
+_get_dtype, _get_shape = attrgetter("dtype"), attrgetter("shape")
+
+
+# torch.cuda.current_stream builds a Stream object first: several times the price of the whole call's checks
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -37,94 +44,94 @@ def _dtype(t: torch.Tensor, name: str) -> int:
     return code
 
 
-class _on:
-    """The tensors' device made current, where it is not, for the library call."""
-
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _call(dev: int, name: str, *args) -> None:
+    """A library call with device ``dev`` current, its current stream as the last argument."""
+    fn = getattr(_lib.load(), name)
+    if dev == torch.cuda.current_device():
+        status = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _stream(dev))
+    if status:
+        _lib.check(status, name)
 
 
 # ---------------------------------------------------------------------------
 # relative attention
 # ---------------------------------------------------------------------------
-def _heads(t, name, b, n, h, d, like):
+_SHORT = 32  # up to here the forward pass has no workspace and keeps nothing for the backward pass
+_INTS = (torch.int32, torch.int64)
+_BOOLS = (torch.bool, torch.uint8)
+
+
+def _heads(t, name, shape, like, dev):
     """A [b, n, h, d] operand of ``like``'s type with the head's values
-    contiguous (copied if they are not), and its (batch, token, head) strides."""
-    if t.shape != (b, n, h, d) or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name}: expected {like.dtype} [{b}, {n}, {h}, {d}] on {like.device}, got {t.dtype} "
+    contiguous (copied if they are not), and its strides."""
+    if t.shape != shape or t.dtype is not like.dtype or t.get_device() != dev:
+        raise ValueError(f"{name}: expected {like.dtype} {list(shape)} on {like.device}, got {t.dtype} "
                          f"{list(t.shape)} on {t.device}")
     st = t.stride()
-    if st[3] != 1 and d > 1:
+    if st[3] != 1 and shape[3] > 1:
         t = t.contiguous()
         st = t.stride()
     return t, st
 
 
-def _tokens(t, name, b, n, dev):
-    if t.shape != (b, n) or t.device != dev or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name}: expected int32 or int64 [{b}, {n}] on {dev}")
-    if t.dtype != torch.int32:
-        t = t.clamp(-(1 << 19), 1 << 19).to(torch.int32)  # the range the operator clamps to
-    return t if n < 2 or t.stride(1) == 1 else t.contiguous()
-
-
 class _Problem:
     """Checked arguments of one call, kept alive with the struct that points at them."""
+
+    __slots__ = ("q", "keep", "tables", "b", "n", "nq", "h", "d", "dev", "arg")
 
     def __init__(self, q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, scale):
         dtype = _dtype(q, "q")
         if q.dim() != 4 or k.dim() != 4:
             raise ValueError("q, k, v: expected [batch, tokens, heads, head_dim]")
-        b, nq, h, d = q.shape
-        n = k.shape[1]
-        dev = q.device
+        b, nq, h, d = shape = q.shape
+        n, dev = k.shape[1], q.get_device()
         if nq > n:
             raise ValueError(f"q has {nq} tokens, k has {n}: the queries are the first tokens")
-        if not 1 <= d <= MAX_HEAD_DIM or h < 1 or h > 65535:
+        if not 1 <= d <= MAX_HEAD_DIM or not 1 <= h <= 65535:
             raise ValueError(f"head_dim: 1 to {MAX_HEAD_DIM}, heads: 1 to 65535 (got {d}, {h})")
-        q, qs = _heads(q, "q", b, nq, h, d, q)
-        k, ks = _heads(k, "k", b, n, h, d, q)
-        v, vs = _heads(v, "v", b, n, h, d, q)
-        tq, tr, tz = (_tokens(t, name, b, n, dev) for t, name in
-                      ((token_q, "token_q"), (token_r, "token_r"), (token_z, "token_z")))
-        m = token_mask
-        if m.shape != (b, n) or m.device != dev or m.dtype not in (torch.bool, torch.uint8):
-            raise ValueError(f"token_mask: expected bool or uint8 [{b}, {n}] on {dev}")
-        if n > 1 and m.stride(1) != 1:
-            m = m.contiguous()
-        clips = []
+        q, qs = _heads(q, "q", shape, q, dev)
+        shape = (b, n, h, d)
+        k, ks = _heads(k, "k", shape, q, dev)
+        v, vs = _heads(v, "v", shape, q, dev)
+        tokens, shape = [], (b, n)
+        for t, kinds, name in ((token_q, _INTS, "token_q"), (token_r, _INTS, "token_r"), (token_z, _INTS, "token_z"),
+                               (token_mask, _BOOLS, "token_mask")):
+            if t.shape != shape or t.get_device() != dev or t.dtype not in kinds:
+                raise ValueError(f"{name}: expected {kinds[0]} or {kinds[1]} [{b}, {n}] on {q.device}")
+            if t.dtype is torch.int64:
+                t = t.clamp(-(1 << 19), 1 << 19).to(torch.int32)  # the range the operator clamps to
+            st = t.stride()
+            if st[1] != 1 and n > 1:
+                t = t.contiguous()
+                st = t.stride()
+            tokens.append(t)
+            tokens.append(st[0])
+        tq, sq, tr, sr, tz, sz, m, sm = tokens
+        td = dq_bias.dtype
+        if td is not torch.float32 and td is not q.dtype:
+            raise ValueError("bias tables: expected float32 or the type of q")
+        rows, tables = [], []
         for t, name, most in ((dq_bias, "dq_bias", MAX_COORD_CLIP), (dr_bias, "dr_bias", MAX_COORD_CLIP),
                               (dz_bias, "dz_bias", MAX_HEIGHT_CLIP)):
-            if t.dim() != 2 or t.shape[1] != h or t.shape[0] % 2 == 0 or t.shape[0] > 2 * most + 1 or t.device != dev:
-                raise ValueError(f"{name}: expected [2 clip + 1, {h}] with clip at most {most} on {dev}")
-            clips.append(t.shape[0] // 2)
-        if clips[0] != clips[1]:
+            ts = t.shape
+            if len(ts) != 2 or ts[1] != h or ts[0] % 2 == 0 or ts[0] > 2 * most + 1 or t.get_device() != dev or \
+                    t.dtype is not td:
+                raise ValueError(f"{name}: expected {td} [2 clip + 1, {h}] with clip at most {most} on {q.device}")
+            rows.append(ts[0])
+            tables.append(t if t.is_contiguous() else t.contiguous())
+        if rows[0] != rows[1]:
             raise ValueError("dq_bias and dr_bias have different clips")
-        tables = [t.contiguous() for t in (dq_bias, dr_bias, dz_bias)]
-        td = tables[0].dtype
-        if td not in (torch.float32, q.dtype) or any(t.dtype != td for t in tables):
-            raise ValueError("bias tables: expected float32 or the type of q, all three alike")
-        self.keep = (q, k, v, tq, tr, tz, m, *tables)
-        self.q, self.table_dtype, self.table_shapes = q, td, [t.shape for t in tables]
-        self.dims, self.dev, self.self_attention = (b, n, nq, h, d), dev, nq == n
-        i3, i4 = C.c_int64 * 3, C.c_int64 * 4
-        self.arg = _lib.HvAttention(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), i3(*qs[:3]), i3(*ks[:3]), i3(*vs[:3]), tq.data_ptr(),
-            tr.data_ptr(), tz.data_ptr(), m.data_ptr(),
-            i4(tq.stride(0), tr.stride(0), tz.stride(0), m.stride(0)), *(t.data_ptr() for t in tables), b, n, nq, h, d,
-            clips[0], clips[2], dtype, _DTYPES[td], float(d ** -0.5 if scale is None else scale))
+        bq, br, bz = tables
+        self.q, self.keep, self.tables = q, (k, v, tq, tr, tz, m), tables
+        self.b, self.n, self.nq, self.h, self.d, self.dev = b, n, nq, h, d, dev
+        self.arg = _lib.pack_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+            tq.data_ptr(), tr.data_ptr(), tz.data_ptr(), m.data_ptr(), sq, sr, sz, sm, bq.data_ptr(), br.data_ptr(),
+            bz.data_ptr(), b, n, nq, h, d, rows[0] // 2, rows[2] // 2, dtype, _DTYPES[td],
+            d ** -0.5 if scale is None else scale)
 
     def sizes(self):
         s = (C.c_size_t * 3)()
@@ -133,7 +140,7 @@ class _Problem:
         return s
 
     def buffer(self, nbytes):
-        return torch.empty((nbytes,), dtype=torch.uint8, device=self.dev) if nbytes else None
+        return torch.empty((nbytes,), dtype=torch.uint8, device=self.q.device) if nbytes else None
 
 
 def _ptr(t):
@@ -157,13 +164,14 @@ def relative_attention_forward(q, k, v, token_q, token_r, token_z, token_mask, d
     :func:`relative_attention_backward`; without ``save`` it is None.
     """
     p = _Problem(q, k, v, token_q, token_r, token_z, token_mask, dq_bias, dr_bias, dz_bias, scale)
-    b, n, nq, h, d = p.dims
-    out = torch.empty((b, nq, h, d), dtype=q.dtype, device=p.dev)
-    with _on(p.dev):
-        sizes = p.sizes()
-        saved, ws = p.buffer(sizes[0] if save else 0), p.buffer(sizes[1])
-        _lib.check(_lib.load().hv_relative_attention_forward(p.arg, out.data_ptr(), _ptr(saved), _ptr(ws), sizes[1],
-                                                             _stream(p.dev)), "relative_attention_forward")
+    out = p.q.new_empty((p.b, p.nq, p.h, p.d))
+    if p.n <= _SHORT:
+        _call(p.dev, "hv_relative_attention_forward", p.arg, out.data_ptr(), None, None, 0)
+        return out, None
+    sizes = p.sizes()
+    saved = p.buffer(sizes[0]) if save else None
+    ws = None if save else p.buffer(sizes[1])
+    _call(p.dev, "hv_relative_attention_forward", p.arg, out.data_ptr(), _ptr(saved), _ptr(ws), sizes[1])
     return out, saved
 
 
@@ -178,30 +186,26 @@ def relative_attention_backward(dout, q, k, v, token_q, token_r, token_z, token_
 
 
 def _backward(p, dout, saved):
-    b, n, nq, h, d = p.dims
-    dout, gs = _heads(dout, "dout", b, nq, h, d, p.q)
-    if p.self_attention:
-        packed = torch.empty((b, n, 3, h, d), dtype=p.q.dtype, device=p.dev)
+    b, n, nq, h, d = p.b, p.n, p.nq, p.h, p.d
+    dout, gs = _heads(dout, "dout", (b, nq, h, d), p.q, p.dev)
+    if nq == n:
+        packed = p.q.new_empty((b, n, 3, h, d))
         dq, dk, dv = packed.unbind(2)
     else:
-        packed = torch.empty((b, n, 2, h, d), dtype=p.q.dtype, device=p.dev)
+        packed = p.q.new_empty((b, n, 2, h, d))
         dk, dv = packed.unbind(2)
-        dq = torch.empty((b, nq, h, d), dtype=p.q.dtype, device=p.dev)
-    tables = [torch.empty(s, dtype=p.table_dtype, device=p.dev) for s in p.table_shapes]
-    i3 = C.c_int64 * 3
-    with _on(p.dev):
-        sizes = p.sizes()
-        if saved is None and sizes[0]:
-            raise ValueError("saved: the forward pass was run without save=True")
-        if saved is not None and saved.numel() != sizes[0]:
-            raise ValueError("saved: not of a forward pass of this shape")
-        ws = p.buffer(sizes[2])
-        gst, dst = i3(*gs[:3]), i3(*dk.stride()[:3])
-        dqs = i3(*dq.stride()[:3])
-        _lib.check(_lib.load().hv_relative_attention_backward(
-            p.arg, dout.data_ptr(), C.addressof(gst), _ptr(saved), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            C.addressof(dqs), C.addressof(dst), *(t.data_ptr() for t in tables), _ptr(ws), sizes[2], _stream(p.dev)),
-            "relative_attention_backward")
+        dq = p.q.new_empty((b, nq, h, d))
+    tables = [torch.empty_like(t) for t in p.tables]
+    sizes = p.sizes()
+    if saved is None and sizes[0]:
+        raise ValueError("saved: the forward pass was run without save=True")
+    if saved is not None and saved.numel() != sizes[0]:
+        raise ValueError("saved: not of a forward pass of this shape")
+    ws = p.buffer(sizes[2])
+    strides = (C.c_int64 * 9)(*gs[:3], *dq.stride()[:3], *dk.stride()[:3])
+    at = C.addressof(strides)
+    _call(p.dev, "hv_relative_attention_backward", p.arg, dout.data_ptr(), at, _ptr(saved), dq.data_ptr(), dk.data_ptr(),
+          dv.data_ptr(), at + 24, at + 48, *(t.data_ptr() for t in tables), _ptr(ws), sizes[2])
     return (dq, dk, dv, *tables), packed
 
 
@@ -256,23 +260,25 @@ def relative_attention_packed(qkv, token_q, token_r, token_z, token_mask, dq_bia
 # ---------------------------------------------------------------------------
 # layer norm
 # ---------------------------------------------------------------------------
-def _rows(t, name, like):
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+def _rows(t, name, like, dev):
+    if t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != dev:
         raise ValueError(f"{name}: expected {like.dtype} {list(like.shape)} on {like.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _norm_params(x, weight, bias):
-    dtype = _dtype(x, "x")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_NORM_WIDTH:
+def _norm_params(x, params):
+    dtype, dev = _dtype(x, "x"), x.get_device()
+    w = x.shape[-1] if x.dim() else 0
+    if not 1 <= w <= MAX_NORM_WIDTH:
         raise ValueError(f"x: the last axis must hold 1 to {MAX_NORM_WIDTH} values")
-    w = x.shape[-1]
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.shape != (w,) or t.device != x.device or t.dtype not in (torch.float32, x.dtype) or t.dtype != weight.dtype:
-            raise ValueError(f"{name}: expected [{w}], float32 or {x.dtype}, on {x.device}")
-    return dtype, w, x.numel() // w
+    kind, out = params[0].dtype, []
+    if kind is not torch.float32 and kind is not x.dtype:
+        raise ValueError(f"weight: expected float32 or {x.dtype}")
+    for t in params:
+        if t.shape != (w,) or t.get_device() != dev or t.dtype is not kind:
+            raise ValueError(f"weight, bias: expected {kind} [{w}] on {x.device}")
+        out.append(t if t.is_contiguous() else t.contiguous())
+    return dtype, dev, w, x.numel() // w, _DTYPES[kind], out
 
 
 def layer_norm_forward(x, weight, bias, eps=1e-5, residual=None):
@@ -280,22 +286,16 @@ def layer_norm_forward(x, weight, bias, eps=1e-5, residual=None):
     returns ``(y, s, mean, rstd)``: s is what was normalised (x itself, or the
     sum in x's type), mean and rstd float32 over the leading axes.  weight and
     bias are float32 or of x's type."""
-    dtype, w, rows = _norm_params(x, weight, bias)
-    x = x if x.is_contiguous() else x.contiguous()
-    dev = x.device
-    s = x
+    dtype, dev, w, rows, kind, (weight, bias) = _norm_params(x, (weight, bias))
+    s = x = x if x.is_contiguous() else x.contiguous()
     if residual is not None:
-        residual = _rows(residual, "residual", x)
+        residual = _rows(residual, "residual", x, dev)
         s = torch.empty_like(x)
     y = torch.empty_like(x)
-    stats = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=dev)
-    mean, rstd = stats.unbind(0)
-    weight, bias = weight.contiguous(), bias.contiguous()
-    with _on(dev):
-        _lib.check(_lib.load().hv_layer_norm_forward(
-            x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), rows, w, dtype, _DTYPES[weight.dtype],
-            eps, None if residual is None else s.data_ptr(), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
-            _stream(dev)), "layer_norm_forward")
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _call(dev, "hv_layer_norm_forward", x.data_ptr(), _ptr(residual), weight.data_ptr(), bias.data_ptr(), rows, w, dtype,
+          kind, eps, None if residual is None else s.data_ptr(), y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, s, mean, rstd
 
 
@@ -304,26 +304,20 @@ def layer_norm_backward(dy, s, weight, mean, rstd, dsum=None):
     where s, mean and rstd are what it returned.  dsum: a gradient that reaches
     s by another way (the residual stream), added into dx; dx is the gradient of
     x and of the residual."""
-    dtype, w, rows = _norm_params(s, weight, None)
-    dy = _rows(dy, "dy", s)
+    dtype, dev, w, rows, kind, (weight,) = _norm_params(s, (weight,))
+    dy = _rows(dy, "dy", s, dev)
     if dsum is not None:
-        dsum = _rows(dsum, "dsum", s)
-    dev = s.device
-    s, weight = s.contiguous(), weight.contiguous()
+        dsum = _rows(dsum, "dsum", s, dev)
+    s = s if s.is_contiguous() else s.contiguous()
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype != torch.float32 or t.shape != s.shape[:-1] or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name}: expected contiguous float32 {list(s.shape[:-1])} on {dev}")
-    dx = torch.empty_like(s)
-    dw, db = torch.empty((2, w), dtype=weight.dtype, device=dev).unbind(0)
-    lib = _lib.load()
-    with _on(dev):
-        need = C.c_size_t(0)
-        _lib.check(lib.hv_layer_norm_workspace_bytes(rows, w, dtype, C.addressof(need)), "layer_norm_workspace_bytes")
-        ws = torch.empty((need.value,), dtype=torch.uint8, device=dev)
-        _lib.check(lib.hv_layer_norm_backward(
-            dy.data_ptr(), s.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(dsum), rows, w,
-            dtype, _DTYPES[weight.dtype], dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need.value,
-            _stream(dev)), "layer_norm_backward")
+        if t.dtype is not torch.float32 or t.shape != s.shape[:-1] or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous float32 {list(s.shape[:-1])} on {s.device}")
+    dx, dw, db = torch.empty_like(s), torch.empty_like(weight), torch.empty_like(weight)
+    need = C.c_size_t(0)
+    _lib.check(_lib.load().hv_layer_norm_workspace_bytes(rows, w, dtype, C.addressof(need)), "layer_norm_workspace_bytes")
+    ws = mean.new_empty((need.value + 3 >> 2,))
+    _call(dev, "hv_layer_norm_backward", dy.data_ptr(), s.data_ptr(), weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+          _ptr(dsum), rows, w, dtype, kind, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ws.data_ptr(), need.value)
     return dx, dw, db
 
 
@@ -379,40 +373,40 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, *, step, lr, betas=(0.9, 0.99
         raise ValueError("step counts from 1")
     if count == 0:
         return
-    first = params[0]
-    dtype, dev, kind = _dtype(first, "params[0]"), first.device, first.dtype
-    total, numel, pp, gp, keep = 0, [], [], [], []
-    for i, (p, g) in enumerate(zip(params, grads)):
-        if p.dtype is not kind or g.dtype is not kind or p.device != dev or g.device != dev or g.shape != p.shape:
-            raise ValueError(f"params[{i}], grads[{i}]: expected {kind} of one shape on {dev}")
-        if not p.is_contiguous():
-            raise ValueError(f"params[{i}]: expected a contiguous tensor")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            keep.append(g)
-        n = p.numel()
-        total += -(-n // STATE_BLOCK) * STATE_BLOCK
-        numel.append(n)
-        pp.append(p.data_ptr())
-        gp.append(g.data_ptr())
+    dtype, dev, kind = _dtype(params[0], "params[0]"), params[0].get_device(), params[0].dtype
+    # whole lists at a time: a network has about a hundred small tensors, and a call of Python for each costs
+    # more than the step
+    tensor = torch.Tensor
+    if set(map(_get_dtype, params)) | set(map(_get_dtype, grads)) != {kind} or \
+            set(map(tensor.get_device, params)) | set(map(tensor.get_device, grads)) != {dev}:
+        raise ValueError(f"params, grads: expected {kind} on {params[0].device}, all of them")
+    shapes = list(map(_get_shape, params))
+    if shapes != list(map(_get_shape, grads)):
+        raise ValueError("params, grads: the shapes differ")
+    if not all(map(tensor.is_contiguous, params)):
+        raise ValueError("params: expected contiguous tensors")
+    if not all(map(tensor.is_contiguous, grads)):
+        grads = [g.contiguous() for g in grads]
+    numel = list(map(tensor.numel, params))
+    total = sum([-(-n // STATE_BLOCK) for n in numel]) * STATE_BLOCK
     want = torch.float32 if scales is None else torch.uint8
     states = [(exp_avg, "exp_avg", want, total), (exp_avg_sq, "exp_avg_sq", want, total)]
     if scales is not None:
         states += [(scales[0], "scales[0]", torch.float32, total // STATE_BLOCK),
                    (scales[1], "scales[1]", torch.float32, total // STATE_BLOCK)]
     for t, name, dt, size in states:
-        if t.dtype is not dt or t.numel() != size or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name}: expected contiguous {dt} of {size} values on {dev}")
+        if t.dtype is not dt or t.numel() != size or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{name}: expected contiguous {dt} of {size} values on {params[0].device}")
     (b1, b2), seed, step = betas, int(seed), int(step)
     key = (seed * 0x6A09E667 + step * 0xBB67AE85) & 0xFFFFFFFF
-    ptrs, sizes = C.c_void_p * count, C.c_int64 * count
-    pa, ga, na = ptrs(*pp), ptrs(*gp), sizes(*numel)
-    with _on(dev):
-        _lib.check(_lib.load().hv_adamw_step(
-            C.addressof(pa), C.addressof(ga), C.addressof(na), count, dtype, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
-            None if scales is None else scales[0].data_ptr(), None if scales is None else scales[1].data_ptr(),
-            32 if scales is None else 8, b1, 1 - b1, b2, 1 - b2, eps, 1 - lr * weight_decay, lr / (1 - b1 ** step),
-            1 / math.sqrt(1 - b2 ** step), key, _stream(dev)), "adamw_step")
+    table = array("q", map(tensor.data_ptr, params))
+    table.extend(map(tensor.data_ptr, grads))
+    table.extend(numel)
+    at = table.buffer_info()[0]
+    _call(dev, "hv_adamw_step", at, at + 8 * count, at + 16 * count, count, dtype, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+          None if scales is None else scales[0].data_ptr(), None if scales is None else scales[1].data_ptr(),
+          32 if scales is None else 8, b1, 1 - b1, b2, 1 - b2, eps, 1 - lr * weight_decay, lr / (1 - b1 ** step),
+          1 / math.sqrt(1 - b2 ** step), key)
 
 
 def _state_values(codes, scale, second):
@@ -421,9 +415,8 @@ def _state_values(codes, scale, second):
     if codes.numel() != scale.numel() * STATE_BLOCK or not codes.is_contiguous() or not scale.is_contiguous():
         raise ValueError(f"expected contiguous codes, {STATE_BLOCK} for each scale")
     out = torch.empty((codes.numel(),), dtype=torch.float32, device=codes.device)
-    with _on(codes.device):
-        _lib.check(_lib.load().hv_adamw_state_values(codes.data_ptr(), scale.data_ptr(), codes.numel(), second,
-                                                     out.data_ptr(), _stream(codes.device)), "adamw_state_values")
+    _call(codes.get_device(), "hv_adamw_state_values", codes.data_ptr(), scale.data_ptr(), codes.numel(), second,
+          out.data_ptr())
     return out
 
 
