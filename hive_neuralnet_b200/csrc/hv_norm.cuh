@@ -19,7 +19,8 @@ namespace hv {
 
 constexpr int kNormThreads = 256;     // rows within a warp
 constexpr int kNormMaxThreads = 512;  // a row in a block
-constexpr int kNormValues = 16;       // values of a row a thread holds at most
+constexpr int kNormValues = 16;       // values of a row a thread holds at most ...
+constexpr int kNormValuesWarp = 8;    // ... where a row lies within a warp
 
 struct NormArgs {
     const void *x, *r, *w, *b;  // b: forward only
@@ -33,124 +34,177 @@ struct NormArgs {
     float eps;
 };
 
-// Sum of a pair of values over the G threads of a row, in all of them.
-__device__ __forceinline__ float2 row_sum(float2 v, int G, float2* scratch) {
-    const int w = G < 32 ? G : 32;
-    for (int o = w >> 1; o; o >>= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+// Sum of a pair of values over the G threads of a row, in all of them.  WIDE:
+// over the block; its warps meet once, two scratch rows take turns.
+template <bool WIDE>
+struct RowSum {
+    float2 (*scratch)[kNormMaxThreads / 32];
+    int G, turn;
+    __device__ __forceinline__ float2 operator()(float2 v) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            if (WIDE || o < G) {
+                v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+                v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+            }
+        if (WIDE) {
+            float2* s = scratch[turn];
+            turn ^= 1;
+            if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+            __syncthreads();
+            const int warps = blockDim.x >> 5;  // a power of two, at most 16
+            v = s[threadIdx.x & (warps - 1)];
+#pragma unroll
+            for (int o = kNormMaxThreads / 64; o; o >>= 1)
+                if (o < warps) {
+                    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+                    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+                }
+        }
+        return v;
     }
-    if (G > 32) {
-        __syncthreads();  // the previous sum's readers are done
-        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-        __syncthreads();
-        v = scratch[0];
-        for (int i = 1; i < (int)(blockDim.x >> 5); i++) v.x += scratch[i].x, v.y += scratch[i].y;
+    __device__ __forceinline__ float operator()(float x) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            if (WIDE || o < G) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (WIDE) {
+            float2* s = scratch[turn];
+            turn ^= 1;
+            if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5].x = x;
+            __syncthreads();
+            const int warps = blockDim.x >> 5;
+            x = s[threadIdx.x & (warps - 1)].x;
+#pragma unroll
+            for (int o = kNormMaxThreads / 64; o; o >>= 1)
+                if (o < warps) x += __shfl_xor_sync(0xffffffffu, x, o);
+        }
+        return x;
     }
-    return v;
-}
+};
 
+// A thread's vectors of a row, K of V values; at: the element offset of the first.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kNormMaxThreads) k_norm_forward(const NormArgs a) {
-    __shared__ float2 scratch[32];
-    const int G = a.G, lane = threadIdx.x & (G - 1), groups = blockDim.x / G, group = threadIdx.x / G;
+struct RowOf {
+    Vec<T, V> x[K];
+    __device__ __forceinline__ void load(const void* base, int64_t at, int step, int left) {
+        const T* p = static_cast<const T*>(base) + at;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (k * step < left) x[k] = *reinterpret_cast<const Vec<T, V>*>(p + k * step);
+    }
+    __device__ __forceinline__ float at(int k, int i) const { return to_f32(x[k].x[i]); }
+};
+
+// Registers: rows within a warp are held to 64, four blocks an SM; wide rows
+// to 128.
+#define HV_NORM_BOUNDS __launch_bounds__(WIDE ? kNormMaxThreads : kNormThreads, WIDE ? 1 : 4)
+
+template <typename T, int V, int K, bool WIDE, bool RES>
+__global__ void HV_NORM_BOUNDS k_norm_forward(const NormArgs a) {
+    __shared__ float2 scratch[2][kNormMaxThreads / 32];
+    const int G = WIDE ? blockDim.x : a.G, lane = threadIdx.x & (G - 1), groups = blockDim.x / G, group = threadIdx.x / G;
+    const int C = a.C, vstep = G * V, left = C - lane * V;  // vector k of a thread is in its row if k vstep < left
+    RowSum<WIDE> row_sum = {scratch, G, 0};
     float w[K][V], b[K][V];
 #pragma unroll
     for (int k = 0; k < K; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = (k * G + lane) * V + i;
-            w[k][i] = c < a.C ? load_param<T>(a.w, c, a.w_f32) : 0.f;
-            b[k][i] = c < a.C ? load_param<T>(a.b, c, a.w_f32) : 0.f;
+            const int c = k * vstep + lane * V + i;
+            w[k][i] = c < C ? load_param<T>(a.w, c, a.w_f32) : 0.f;
+            b[k][i] = c < C ? load_param<T>(a.b, c, a.w_f32) : 0.f;
         }
-    const float inv_c = 1.f / (float)a.C;
+    const float inv_c = 1.f / (float)C;
+    const int64_t step = (int64_t)gridDim.x * groups, astep = step * C;
+    int64_t row = (int64_t)blockIdx.x * groups + group, at = row * C + lane * V;
+    RowOf<T, V, K> x, r;
+    if (row < a.rows) {
+        x.load(a.x, at, vstep, left);
+        if (RES) r.load(a.r, at, vstep, left);
+    }
     // whole groups of rows, so that every thread of a warp reaches the shuffles
-    const int64_t step = (int64_t)gridDim.x * groups;
     for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += step) {
-        const int64_t row = r0 + group;
         const bool live = row < a.rows;
-        const T* x = static_cast<const T*>(a.x) + row * a.C;
-        float v[K][V];
-        float2 sum = make_float2(0.f, 0.f);
+        float v[K][V], sum = 0.f;
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int c = (k * G + lane) * V;
-            const bool in = live && c < a.C;
+            const bool in = live && k * vstep < left;
 #pragma unroll
-            for (int i = 0; i < V; i++) v[k][i] = 0.f;
-            if (in) {
-                load_vec<T, V>(x + c, v[k]);
-                if (a.r) {
-                    float r[V];
-                    load_vec<T, V>(static_cast<const T*>(a.r) + row * a.C + c, r);
-#pragma unroll
-                    for (int i = 0; i < V; i++) v[k][i] = to_f32(from_f32<T>(v[k][i] + r[i]));
-                    store_vec<T, V>(static_cast<T*>(a.s) + row * a.C + c, v[k]);
-                }
+            for (int i = 0; i < V; i++) {
+                v[k][i] = x.at(k, i);
+                if (RES) v[k][i] = to_f32(from_f32<T>(v[k][i] + r.at(k, i)));
+                v[k][i] = in ? v[k][i] : 0.f;
+                sum += v[k][i];
             }
-#pragma unroll
-            for (int i = 0; i < V; i++) sum.x += v[k][i];
+            if (RES && in) store_vec<T, V>(static_cast<T*>(a.s) + at + k * vstep, v[k]);
         }
-        const float mean = row_sum(sum, G, scratch).x * inv_c;
-        sum = make_float2(0.f, 0.f);
+        if (row + step < a.rows) {  // the next row's, a turn ahead
+            x.load(a.x, at + astep, vstep, left);
+            if (RES) r.load(a.r, at + astep, vstep, left);
+        }
+        const float mean = row_sum(sum) * inv_c;
+        sum = 0.f;
 #pragma unroll
         for (int k = 0; k < K; k++)
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                v[k][i] = (k * G + lane) * V + i < a.C ? v[k][i] - mean : 0.f;
-                sum.x = fmaf(v[k][i], v[k][i], sum.x);
+                v[k][i] = k * vstep < left ? v[k][i] - mean : 0.f;
+                sum = fmaf(v[k][i], v[k][i], sum);
             }
-        const float rstd = 1.f / sqrtf(row_sum(sum, G, scratch).x * inv_c + a.eps);
-        if (!live) continue;
-        T* y = static_cast<T*>(a.y) + row * a.C;
+        const float rstd = rsqrtf(row_sum(sum) * inv_c + a.eps);
+        if (live) {
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int c = (k * G + lane) * V;
-            if (c >= a.C) continue;
-            float o[V];
+            for (int k = 0; k < K; k++) {
+                if (k * vstep >= left) continue;
+                float o[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
-            store_vec<T, V>(y + c, o);
+                for (int i = 0; i < V; i++) o[i] = fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
+                store_vec<T, V>(static_cast<T*>(a.y) + at + k * vstep, o);
+            }
+            if (lane == 0 && a.mean) a.mean[row] = mean, a.rstd[row] = rstd;
         }
-        if (lane == 0 && a.mean) a.mean[row] = mean, a.rstd[row] = rstd;
+        row += step, at += astep;
     }
 }
 
-template <typename T, int V, int K>
-__global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArgs a) {
-    __shared__ float2 scratch[32];
-    __shared__ float part[kNormThreads * V];
-    const int G = a.G, lane = threadIdx.x & (G - 1), groups = blockDim.x / G, group = threadIdx.x / G;
+template <typename T, int V, int K, bool WIDE, bool RES>
+__global__ void HV_NORM_BOUNDS k_norm_backward(const NormArgs a) {
+    __shared__ float2 scratch[2][kNormMaxThreads / 32];
+    __shared__ float part[WIDE ? 1 : kNormThreads * V];
+    const int G = WIDE ? blockDim.x : a.G, lane = threadIdx.x & (G - 1), groups = blockDim.x / G, group = threadIdx.x / G;
+    const int C = a.C, vstep = G * V, left = C - lane * V;
+    RowSum<WIDE> row_sum = {scratch, G, 0};
     float w[K][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = (k * G + lane) * V + i;
-            w[k][i] = c < a.C ? load_param<T>(a.w, c, a.w_f32) : 0.f;
+            const int c = k * vstep + lane * V + i;
+            w[k][i] = c < C ? load_param<T>(a.w, c, a.w_f32) : 0.f;
             dw[k][i] = db[k][i] = 0.f;
         }
-    const float inv_c = 1.f / (float)a.C;
-    const int64_t step = (int64_t)gridDim.x * groups;
+    const float inv_c = 1.f / (float)C;
+    const int64_t step = (int64_t)gridDim.x * groups, astep = step * C;
+    int64_t row = (int64_t)blockIdx.x * groups + group, at = row * C + lane * V;
     for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += step) {
-        const int64_t row = r0 + group;
         const bool live = row < a.rows;
-        const float mean = live ? a.mean[row] : 0.f, rstd = live ? a.rstd[row] : 0.f;
+        RowOf<T, V, K> x, dy, ds;
+        float mean = 0.f, rstd = 0.f;
+        if (live) {
+            x.load(a.x, at, vstep, left);
+            dy.load(a.dy, at, vstep, left);
+            if (RES) ds.load(a.ds, at, vstep, left);
+            mean = a.mean[row], rstd = a.rstd[row];
+        }
         float xh[K][V], g[K][V];
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const int c = (k * G + lane) * V;
-            if (live && c < a.C) {
-                load_vec<T, V>(static_cast<const T*>(a.x) + row * a.C + c, xh[k]);
-                load_vec<T, V>(static_cast<const T*>(a.dy) + row * a.C + c, g[k]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) xh[k][i] = mean, g[k][i] = 0.f;
-            }
+            const bool in = live && k * vstep < left;
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                xh[k][i] = (xh[k][i] - mean) * rstd;
+                xh[k][i] = in ? (x.at(k, i) - mean) * rstd : 0.f;
+                g[k][i] = in ? dy.at(k, i) : 0.f;
                 db[k][i] += g[k][i];
                 dw[k][i] = fmaf(g[k][i], xh[k][i], dw[k][i]);
                 g[k][i] *= w[k][i];
@@ -158,24 +212,21 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
                 sum.y = fmaf(g[k][i], xh[k][i], sum.y);
             }
         }
-        sum = row_sum(sum, G, scratch);
+        sum = row_sum(sum);
         const float mg = sum.x * inv_c, mgx = sum.y * inv_c;
-        if (!live) continue;
+        if (live)
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const int c = (k * G + lane) * V;
-            if (c >= a.C) continue;
-            float o[V];
+            for (int k = 0; k < K; k++) {
+                if (k * vstep >= left) continue;
+                float o[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = rstd * (g[k][i] - mg - xh[k][i] * mgx);
-            if (a.ds) {
-                float d[V];
-                load_vec<T, V>(static_cast<const T*>(a.ds) + row * a.C + c, d);
-#pragma unroll
-                for (int i = 0; i < V; i++) o[i] += d[i];
+                for (int i = 0; i < V; i++) {
+                    o[i] = rstd * (g[k][i] - mg - xh[k][i] * mgx);
+                    if (RES) o[i] += ds.at(k, i);
+                }
+                store_vec<T, V>(static_cast<T*>(a.dx) + at + k * vstep, o);
             }
-            store_vec<T, V>(static_cast<T*>(a.dx) + row * a.C + c, o);
-        }
+        row += step, at += astep;
     }
     // this block's sums over its rows, in a fixed order: over the groups of a
     // warp by shuffles, over the warps through shared memory
@@ -187,7 +238,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
         else
             out[which * a.C + c] = x;
     };
-    const int span = G < 32 ? G : 32, warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
 #pragma unroll
     for (int which = 0; which < 2; which++)
 #pragma unroll
@@ -196,13 +247,14 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 v[i] = which ? db[k][i] : dw[k][i];
-                for (int o = span; o < 32; o <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+                if (!WIDE)
+                    for (int o = G; o < 32; o <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
             }
-            if (G > 32) {  // one row a block: its threads own their columns
-                const int c = (k * G + lane) * V;
+            if (WIDE) {  // one row a block: its threads own their columns
+                const int c = k * vstep + lane * V;
 #pragma unroll
                 for (int i = 0; i < V; i++)
-                    if (c + i < a.C) put(which, c + i, v[i]);
+                    if (c + i < C) put(which, c + i, v[i]);
                 continue;
             }
             __syncthreads();
@@ -214,10 +266,12 @@ __global__ void __launch_bounds__(kNormMaxThreads) k_norm_backward(const NormArg
                 float t = 0.f;
                 for (int q = 0; q < (int)(blockDim.x >> 5); q++) t += part[q * G * V + j];
                 const int c = k * G * V + j;
-                if (c < a.C) put(which, c, t);
+                if (c < C) put(which, c, t);
             }
         }
 }
+
+#undef HV_NORM_BOUNDS
 
 // Sums the blocks' partial rows [n][2][C] into dw and db: 32 columns a block,
 // 32 threads down each column.
@@ -228,6 +282,7 @@ __global__ void __launch_bounds__(1024) k_norm_reduce(const float* __restrict__ 
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     float v = 0.f;
     if (col < 2 * C)
+#pragma unroll 8
         for (int i = part; i < n; i += 32) v += partial[(int64_t)i * 2 * C + col];
     t[part][threadIdx.x & 31] = v;
     __syncthreads();

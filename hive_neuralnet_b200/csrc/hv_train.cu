@@ -35,6 +35,30 @@ static int sm_count() {
     return n[dev];
 }
 
+constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024;
+
+// Shared-memory limit and resident blocks of a kernel, asked for once per
+// device and shape.
+template <typename K>
+static int resident_blocks(K kernel, int threads, int smem, int* out) {
+    struct Known { int threads, smem, blocks; };
+    static Known known[64];
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HV_ECUDA;
+    std::lock_guard<std::mutex> lock(mu);
+    Known& k = known[dev];
+    if (!k.blocks || k.threads != threads || k.smem != smem) {
+        if (smem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock) != cudaSuccess)
+            return HV_ECUDA;
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return HV_ECUDA;
+        k = {threads, smem, n};
+    }
+    *out = k.blocks;
+    return HV_OK;
+}
+
 // Calls f with a value of the element type.
 template <typename F>
 static int by_type(int dtype, F f) {
@@ -50,29 +74,32 @@ static int by_type(int dtype, F f) {
 // layer norm
 // ---------------------------------------------------------------------------
 constexpr int kNormMaxWidth = kNormMaxThreads * kNormValues;
-constexpr int kNormBlocksPerSm = 4;
+constexpr int kNormBlocksPerSm = 8;  // at most
 
 struct NormShape {
     int V, K, G, threads;
+    bool wide;
 };
 
 // V values a vector where rows and pointers allow 16-byte vectors, else 1.  A
-// row goes to the fewest threads of a warp that hold it at up to 16 values
-// each, or to a block where a warp cannot hold it.
+// row goes to the fewest threads of a warp that hold it at 8 values each (the
+// more values a thread, the fewer shuffles a value), or to a block.
 static bool norm_shape(int C, int dtype, bool vec, NormShape* s) {
     s->V = vec ? (int)(16 / elem_bytes(dtype)) : 1;
     const int n = (C + s->V - 1) / s->V;  // vectors of a row
-    s->G = 1;
-    while (s->G < 32 && s->G < n) s->G *= 2;
-    s->threads = kNormThreads;
-    if (n * s->V > 32 * kNormValues) {
+    s->wide = C > 32 * kNormValuesWarp;
+    if (s->wide) {
         s->threads = 128;
         while (s->threads < kNormMaxThreads && n * s->V > s->threads * (kNormValues / 2)) s->threads *= 2;
         s->G = s->threads;
+    } else {
+        s->threads = kNormThreads;
+        s->G = 1;
+        while (n * s->V > s->G * kNormValuesWarp) s->G *= 2;
     }
     s->K = 1;
     while (s->K * s->G < n) s->K *= 2;
-    return s->K * s->V <= kNormValues;
+    return s->K * s->V <= (s->wide ? kNormValues : kNormValuesWarp);
 }
 
 static bool norm_vec(int C, int dtype, std::initializer_list<const void*> ptrs) {
@@ -81,37 +108,47 @@ static bool norm_vec(int C, int dtype, std::initializer_list<const void*> ptrs) 
     return ok;
 }
 
-template <typename T, bool BACK>
-static int launch_norm(const NormArgs& a, const NormShape& s, int grid, cudaStream_t st) {
-    auto go = [&](auto kernel) {
-        kernel<<<grid, s.threads, 0, st>>>(a);
-        return launched();
-    };
-    constexpr int V = 16 / sizeof(T);
-#define HV_NORM(VV, KK)                                        \
-    if constexpr (VV * KK <= kNormValues)                      \
-        if (s.V == VV && s.K == KK) {                          \
-            if constexpr (BACK) return go(k_norm_backward<T, VV, KK>); \
-            else return go(k_norm_forward<T, VV, KK>);         \
-        }
-    HV_NORM(V, 1)
-    HV_NORM(V, 2)
-    HV_NORM(V, 4)
-    HV_NORM(1, 1)
-    HV_NORM(1, 2)
-    HV_NORM(1, 4)
-    HV_NORM(1, 8)
-    HV_NORM(1, 16)
-#undef HV_NORM
-    return HV_EINVAL;
+static int norm_blocks(const NormShape& s, int64_t rows, int resident) {
+    const int64_t blocks = (rows + s.threads / s.G - 1) / (s.threads / s.G), cap = (int64_t)sm_count() * resident;
+    return (int)(blocks < cap ? blocks : cap);
 }
 
 // Backward: up to four turns of one block cost less than a second launch that
 // joins several blocks' sums.
-static int norm_grid(const NormShape& s, int64_t rows, bool back) {
-    if (back && rows <= 4 * (s.threads / s.G)) return 1;
-    const int64_t blocks = (rows + s.threads / s.G - 1) / (s.threads / s.G), cap = (int64_t)sm_count() * kNormBlocksPerSm;
-    return (int)(blocks < cap ? blocks : cap);
+static bool norm_one_block(const NormShape& s, int64_t rows) { return rows <= 4 * (s.threads / s.G); }
+
+// grid: the blocks launched
+template <typename T, bool BACK, bool RES>
+static int launch_norm(const NormArgs& a, const NormShape& s, int* grid, cudaStream_t st) {
+    auto go = [&](auto kernel) -> int {
+        int n = 0;
+        const int rc = resident_blocks(kernel, s.threads, 0, &n);
+        if (rc) return rc;
+        *grid = BACK && norm_one_block(s, a.rows) ? 1 : norm_blocks(s, a.rows, n < kNormBlocksPerSm ? n : kNormBlocksPerSm);
+        kernel<<<*grid, s.threads, 0, st>>>(a);
+        return launched();
+    };
+    constexpr int V = 16 / sizeof(T);
+#define HV_NORM(VV, KK, WW)                                                    \
+    if constexpr (VV * KK <= (WW ? kNormValues : kNormValuesWarp))             \
+        if (s.V == VV && s.K == KK && s.wide == WW) {                          \
+            if constexpr (BACK) return go(k_norm_backward<T, VV, KK, WW, RES>); \
+            else return go(k_norm_forward<T, VV, KK, WW, RES>);                \
+        }
+    HV_NORM(V, 1, false)
+    HV_NORM(V, 2, false)
+    HV_NORM(1, 1, false)
+    HV_NORM(1, 2, false)
+    HV_NORM(1, 4, false)
+    HV_NORM(1, 8, false)
+    HV_NORM(V, 1, true)
+    HV_NORM(V, 2, true)
+    HV_NORM(V, 4, true)
+    HV_NORM(1, 4, true)
+    HV_NORM(1, 8, true)
+    HV_NORM(1, 16, true)
+#undef HV_NORM
+    return HV_EINVAL;
 }
 
 // ---------------------------------------------------------------------------
@@ -135,7 +172,7 @@ static bool attn_ok(const hv_attention* a) {
 static int attn_classes(const hv_attention* a) { return 2 * (2 * a->coord_clip + 1) + 2 * a->height_clip + 1; }
 
 // ---- up to 32 tokens
-constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024, kShortSmem = 100 * 1024;
+constexpr int kShortSmem = 100 * 1024;
 
 static bool attn_short(const hv_attention* a) { return a->tokens <= kSlots; }
 
@@ -171,28 +208,6 @@ static int short_blocks(const ShortPlan& p, int64_t batch, int resident) {
 static int short_resident(const ShortPlan& p) {  // at most, on an SM
     const int by_smem = kSmemPerSm / (p.total + 1024), by_threads = 64 / p.HG;
     return by_smem < by_threads ? (by_smem < 32 ? by_smem : 32) : (by_threads < 32 ? by_threads : 32);
-}
-
-// Shared-memory limit and resident blocks of a kernel, asked for once per
-// device and shape.
-template <typename K>
-static int resident_blocks(K kernel, int threads, int smem, int* out) {
-    struct Known { int threads, smem, blocks; };
-    static Known known[64];
-    static std::mutex mu;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HV_ECUDA;
-    std::lock_guard<std::mutex> lock(mu);
-    Known& k = known[dev];
-    if (!k.blocks || k.threads != threads || k.smem != smem) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock) != cudaSuccess)
-            return HV_ECUDA;
-        int n = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return HV_ECUDA;
-        k = {threads, smem, n};
-    }
-    *out = k.blocks;
-    return HV_OK;
 }
 
 template <typename T, bool BACK>
@@ -357,15 +372,19 @@ int hv_layer_norm_forward(const void* x, const void* residual, const void* weigh
     NormArgs a = {};
     a.x = x, a.r = residual, a.w = weight, a.b = bias, a.s = sum, a.y = y, a.mean = mean, a.rstd = rstd;
     a.rows = rows, a.C = width, a.G = s.G, a.w_f32 = weight_dtype == HV_F32, a.eps = eps;
-    const int grid = norm_grid(s, rows, false);
-    return by_type(dtype, [&](auto t) { return launch_norm<decltype(t), false>(a, s, grid, (cudaStream_t)stream); });
+    int grid = 0;
+    return by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        return residual ? launch_norm<T, false, true>(a, s, &grid, (cudaStream_t)stream)
+                        : launch_norm<T, false, false>(a, s, &grid, (cudaStream_t)stream);
+    });
 }
 
 int hv_layer_norm_workspace_bytes(int64_t rows, int width, int dtype, size_t* bytes) {
     NormShape s, t;
     if (!bytes || rows < 0 || width < 1 || width > kNormMaxWidth || dtype < 0 || dtype > 2) return HV_EINVAL;
     if (!norm_shape(width, dtype, false, &s) || !norm_shape(width, dtype, true, &t)) return HV_EINVAL;
-    const int g = norm_grid(s, rows, true), h = norm_grid(t, rows, true);
+    const int g = norm_blocks(s, rows, kNormBlocksPerSm), h = norm_blocks(t, rows, kNormBlocksPerSm);
     *bytes = (size_t)(g > h ? g : h) * 2 * width * 4;
     if (*bytes < 16) *bytes = 16;
     return HV_OK;
@@ -380,8 +399,7 @@ int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     if (rows && (!dy || !x || !weight || !mean || !rstd || !dx)) return HV_EINVAL;
     NormShape s;
     if (!norm_shape(width, dtype, norm_vec(width, dtype, {dy, x, dsum, dx}), &s)) return HV_EINVAL;
-    const int grid = rows ? norm_grid(s, rows, true) : 0;
-    if (workspace_bytes < (size_t)grid * 2 * width * 4) return HV_EINVAL;
+    if (workspace_bytes < (size_t)norm_blocks(s, rows, kNormBlocksPerSm) * 2 * width * 4) return HV_EINVAL;
     NormArgs a = {};
     a.x = x, a.w = weight, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
     a.dy = dy, a.ds = dsum, a.dx = dx, a.dw = dweight, a.db = dbias, a.partial = static_cast<float*>(workspace);
@@ -389,8 +407,9 @@ int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     const cudaStream_t st = (cudaStream_t)stream;
     return by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        if (grid) {
-            const int rc = launch_norm<T, true>(a, s, grid, st);
+        int grid = 0;
+        if (rows) {
+            const int rc = dsum ? launch_norm<T, true, true>(a, s, &grid, st) : launch_norm<T, true, false>(a, s, &grid, st);
             if (rc || grid == 1) return rc;
         }
         k_norm_reduce<T><<<(2 * width + 31) / 32, 1024, 0, st>>>(a.partial, grid, width, dweight, dbias, a.w_f32);
