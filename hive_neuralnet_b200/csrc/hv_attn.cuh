@@ -46,20 +46,25 @@ __global__ void __launch_bounds__(1024) k_attn_table_sum(const float* __restrict
     const int v = threadIdx.x & 7, part = threadIdx.x >> 3, at = blockIdx.x * 8 + v, values = classes * H;
     float x = 0.f;
     if (at < values)
+#pragma unroll 4
         for (int64_t i = part; i < n; i += 128) x += partial[i * values + at];
     x += __shfl_xor_sync(0xffffffffu, x, 8);
     x += __shfl_xor_sync(0xffffffffu, x, 16);
     if ((threadIdx.x & 31) < 8) sums[threadIdx.x >> 5][v] = x;
     __syncthreads();
-    if (threadIdx.x >= 8 || at >= values) return;
-    x = 0.f;
-    for (int i = 0; i < 32; i++) x += sums[i][v];
-    if (at < W * H)
-        store_param<T>(dbq, at, t_f32, x);
-    else if (at < 2 * W * H)
-        store_param<T>(dbr, at - W * H, t_f32, x);
+    if (threadIdx.x >= 256) return;
+    // warp c: value c's 32 sums
+    x = sums[threadIdx.x & 31][threadIdx.x >> 5];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    const int c = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if ((threadIdx.x & 31) || c >= values) return;
+    if (c < W * H)
+        store_param<T>(dbq, c, t_f32, x);
+    else if (c < 2 * W * H)
+        store_param<T>(dbr, c - W * H, t_f32, x);
     else
-        store_param<T>(dbz, at - 2 * W * H, t_f32, x);
+        store_param<T>(dbz, c - 2 * W * H, t_f32, x);
 }
 
 }  // namespace hv

@@ -44,6 +44,27 @@ __device__ __forceinline__ void store_vec(T* p, const float* in) {
     *reinterpret_cast<Vec<T, N>*>(p) = v;
 }
 
+// A pair of fp32 values in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 c;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{ .reg .b64 w, x, y, z; mov.b64 w, {%2, %3}; mov.b64 x, {%4, %5}; mov.b64 y, {%6, %7}; fma.rn.f32x2 z, w, x, y; "
+        "mov.b64 {%0, %1}, z; }"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
 // A value of a small fp32-or-T parameter tensor (weights, bias tables).
 template <typename T>
 __device__ __forceinline__ float load_param(const void* p, int64_t i, bool is_f32) {

@@ -59,27 +59,6 @@ __device__ __forceinline__ float2 unpack2(uint32_t x, __nv_bfloat16) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
 }
 
-// A pair of fp32 values in one instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 c;
-    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
-        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return c;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 c;
-    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }"
-        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return c;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{ .reg .b64 w, x, y, z; mov.b64 w, {%2, %3}; mov.b64 x, {%4, %5}; mov.b64 y, {%6, %7}; fma.rn.f32x2 z, w, x, y; "
-        "mov.b64 {%0, %1}, z; }"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-
 // c = a b + (FIRST ? 0 : c)
 #define HV_MMA(NAME, SHAPE, TYPES, NA, AREGS, BREGS)                                                                    \
     template <bool FIRST>                                                                                               \

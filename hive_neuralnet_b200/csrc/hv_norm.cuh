@@ -17,10 +17,10 @@
 
 namespace hv {
 
-constexpr int kNormThreads = 256;     // rows within a warp
+constexpr int kNormThreads = 256;    // rows within a warp
 constexpr int kNormMaxThreads = 512;  // a row in a block
-constexpr int kNormValues = 16;       // values of a row a thread holds at most ...
-constexpr int kNormValuesWarp = 8;    // ... where a row lies within a warp
+constexpr int kNormValues = 8;        // values of a row a thread holds at most ...
+constexpr int kNormValuesWide = 16;   // ... where it takes a block
 
 struct NormArgs {
     const void *x, *r, *w, *b;  // b: forward only
@@ -34,199 +34,283 @@ struct NormArgs {
     float eps;
 };
 
-// Sum of a pair of values over the G threads of a row, in all of them.  WIDE:
-// over the block; its warps meet once, two scratch rows take turns.
-template <bool WIDE>
+// How a row is spread.  LG >= 0: over 2^LG threads of a warp; kLoose: over G
+// threads of a warp, G known at run time; kWide: over the block.
+constexpr int kLoose = -1, kWide = -2;
+
+// Sum of a value or a pair over the threads of a row, in all of them.  A
+// block's warps meet once; two scratch rows take turns.
+__device__ __forceinline__ float2 plus(float2 a, float2 b) { return add2(a, b); }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float2 shuffled(float2 v, int o) {
+    return make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o));
+}
+__device__ __forceinline__ float shuffled(float v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+
+template <int LG>
 struct RowSum {
     float2 (*scratch)[kNormMaxThreads / 32];
     int G, turn;
-    __device__ __forceinline__ float2 operator()(float2 v) {
+    template <typename X>
+    __device__ __forceinline__ X operator()(X v) {
 #pragma unroll
         for (int o = 16; o; o >>= 1)
-            if (WIDE || o < G) {
-                v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-                v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-            }
-        if (WIDE) {
-            float2* s = scratch[turn];
+            if (LG >= 0 ? o < (1 << (LG < 0 ? 0 : LG)) : LG == kWide || o < G) v = plus(v, shuffled(v, o));
+        if (LG == kWide) {
+            X* s = reinterpret_cast<X*>(scratch[turn]);
             turn ^= 1;
             if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
             __syncthreads();
-            const int warps = blockDim.x >> 5;  // a power of two, at most 16
+            const int warps = blockDim.x >> 5;  // a power of two
             v = s[threadIdx.x & (warps - 1)];
 #pragma unroll
             for (int o = kNormMaxThreads / 64; o; o >>= 1)
-                if (o < warps) {
-                    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-                    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-                }
+                if (o < warps) v = plus(v, shuffled(v, o));
         }
         return v;
     }
-    __device__ __forceinline__ float operator()(float x) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1)
-            if (WIDE || o < G) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (WIDE) {
-            float2* s = scratch[turn];
-            turn ^= 1;
-            if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5].x = x;
-            __syncthreads();
-            const int warps = blockDim.x >> 5;
-            x = s[threadIdx.x & (warps - 1)].x;
-#pragma unroll
-            for (int o = kNormMaxThreads / 64; o; o >>= 1)
-                if (o < warps) x += __shfl_xor_sync(0xffffffffu, x, o);
-        }
-        return x;
-    }
 };
 
-// A thread's vectors of a row, K of V values; at: the element offset of the first.
+// A thread's vectors of a row, K of V values.
 template <typename T, int V, int K>
 struct RowOf {
     Vec<T, V> x[K];
-    __device__ __forceinline__ void load(const void* base, int64_t at, int step, int left) {
-        const T* p = static_cast<const T*>(base) + at;
+    // row: the row's (the thread's) first value; vector k lies k step values on, in the row if that is below left
+    __device__ __forceinline__ void load(const T* row, uint32_t at, uint32_t step, int left) {
 #pragma unroll
         for (int k = 0; k < K; k++)
-            if (k * step < left) x[k] = *reinterpret_cast<const Vec<T, V>*>(p + k * step);
+            if ((int)(k * step) < left) x[k] = *reinterpret_cast<const Vec<T, V>*>(row + (at + k * step));
     }
-    __device__ __forceinline__ float at(int k, int i) const { return to_f32(x[k].x[i]); }
+    __device__ __forceinline__ float2 pair(int k, int i) const { return make_float2(to_f32(x[k].x[i]), to_f32(x[k].x[i + 1])); }
+    __device__ __forceinline__ float one(int k, int i) const { return to_f32(x[k].x[i]); }
 };
 
-// Registers: rows within a warp are held to 64, four blocks an SM; wide rows
-// to 128.
-#define HV_NORM_BOUNDS __launch_bounds__(WIDE ? kNormMaxThreads : kNormThreads, WIDE ? 1 : 4)
+// Elementwise steps on V values, in pairs where there are pairs.
+template <int V, typename F2, typename F1>
+__device__ __forceinline__ void by_pairs(F2 two, F1 one) {
+    if constexpr (V == 1) {
+        one(0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) two(i);
+    }
+}
 
-template <typename T, int V, int K, bool WIDE, bool RES>
-__global__ void HV_NORM_BOUNDS k_norm_forward(const NormArgs a) {
-    __shared__ float2 scratch[2][kNormMaxThreads / 32];
-    const int G = WIDE ? blockDim.x : a.G, lane = threadIdx.x & (G - 1), groups = blockDim.x / G, group = threadIdx.x / G;
-    const int C = a.C, vstep = G * V, left = C - lane * V;  // vector k of a thread is in its row if k vstep < left
-    RowSum<WIDE> row_sum = {scratch, G, 0};
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Registers for BLOCKS blocks of 256 threads an SM; wide rows as they come.
+#define HV_NORM_BOUNDS(BLOCKS) __launch_bounds__(LG == kWide ? kNormMaxThreads : kNormThreads, LG == kWide ? 1 : BLOCKS)
+
+// What both passes set up: the threads of a row, this thread's place, its rows.
+#define HV_NORM_PLACE                                                                                               \
+    __shared__ float2 scratch[2][kNormMaxThreads / 32];                                                             \
+    const int G = LG == kWide ? blockDim.x : LG >= 0 ? 1 << (LG < 0 ? 0 : LG) : a.G;                                \
+    const int lane = threadIdx.x & (G - 1), groups = LG == kWide ? 1 : blockDim.x / G, group = LG == kWide ? 0 : threadIdx.x / G; \
+    const int C = a.C, left = C - lane * V;                                                                         \
+    const uint32_t vstep = G * V, at = lane * V;                                                                    \
+    RowSum<LG> row_sum = {scratch, G, 0};                                                                           \
+    const float inv_c = 1.f / (float)C;                                                                             \
+    const int64_t step = (int64_t)gridDim.x * groups, astep = step * C;                                             \
+    int64_t r0 = (int64_t)blockIdx.x * groups, row = r0 + group, first = row * C;
+
+template <typename T, int V, int K, int LG, bool RES>
+__global__ void HV_NORM_BOUNDS(4) k_norm_forward(const NormArgs a) {
+    HV_NORM_PLACE
+    const bool full = (int)(K * vstep) == C;  // every vector of every thread lies in the row
     float w[K][V], b[K][V];
 #pragma unroll
     for (int k = 0; k < K; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = k * vstep + lane * V + i;
+            const int c = k * vstep + at + i;
             w[k][i] = c < C ? load_param<T>(a.w, c, a.w_f32) : 0.f;
             b[k][i] = c < C ? load_param<T>(a.b, c, a.w_f32) : 0.f;
         }
-    const float inv_c = 1.f / (float)C;
-    const int64_t step = (int64_t)gridDim.x * groups, astep = step * C;
-    int64_t row = (int64_t)blockIdx.x * groups + group, at = row * C + lane * V;
-    RowOf<T, V, K> x, r;
+    const T *px = static_cast<const T*>(a.x) + first, *pr = static_cast<const T*>(a.r) + (RES ? first : 0);
+    T *py = static_cast<T*>(a.y) + first, *ps = static_cast<T*>(a.s) + (RES ? first : 0);
+    RowOf<T, V, K> x = {}, r = {};
     if (row < a.rows) {
-        x.load(a.x, at, vstep, left);
-        if (RES) r.load(a.r, at, vstep, left);
+        x.load(px, at, vstep, left);
+        if (RES) r.load(pr, at, vstep, left);
     }
     // whole groups of rows, so that every thread of a warp reaches the shuffles
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += step) {
+    for (; r0 < a.rows; r0 += step) {
         const bool live = row < a.rows;
         float v[K][V], sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            const bool in = live && k * vstep < left;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                v[k][i] = x.at(k, i);
-                if (RES) v[k][i] = to_f32(from_f32<T>(v[k][i] + r.at(k, i)));
-                v[k][i] = in ? v[k][i] : 0.f;
-                sum += v[k][i];
-            }
-            if (RES && in) store_vec<T, V>(static_cast<T*>(a.s) + at + k * vstep, v[k]);
+        for (int k = 0; k < K; k++) {  // past the row's end: zeros
+            Vec<T, V> s;
+            by_pairs<V>(
+                [&](int i) {
+                    float2 z = x.pair(k, i);
+                    if (RES) {
+                        z = add2(z, r.pair(k, i));
+                        s.x[i] = from_f32<T>(z.x), s.x[i + 1] = from_f32<T>(z.y);
+                        z = make_float2(to_f32(s.x[i]), to_f32(s.x[i + 1]));
+                    }
+                    v[k][i] = z.x, v[k][i + 1] = z.y;
+                    sum += z.x + z.y;
+                },
+                [&](int) {
+                    v[k][0] = x.one(k, 0);
+                    if (RES) s.x[0] = from_f32<T>(v[k][0] + r.one(k, 0)), v[k][0] = to_f32(s.x[0]);
+                    sum += v[k][0];
+                });
+            if (RES && live && (int)(k * vstep) < left) *reinterpret_cast<Vec<T, V>*>(ps + (at + k * vstep)) = s;
         }
         if (row + step < a.rows) {  // the next row's, a turn ahead
-            x.load(a.x, at + astep, vstep, left);
-            if (RES) r.load(a.r, at + astep, vstep, left);
+            x.load(px + astep, at, vstep, left);
+            if (RES) r.load(pr + astep, at, vstep, left);
         }
         const float mean = row_sum(sum) * inv_c;
-        sum = 0.f;
+        float2 squares = both(0.f);
 #pragma unroll
         for (int k = 0; k < K; k++)
+            by_pairs<V>(
+                [&](int i) {
+                    const float2 z = add2(make_float2(v[k][i], v[k][i + 1]), both(-mean));
+                    v[k][i] = z.x, v[k][i + 1] = z.y;
+                },
+                [&](int) { v[k][0] -= mean; });
+        if (!full)
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                v[k][i] = k * vstep < left ? v[k][i] - mean : 0.f;
-                sum = fmaf(v[k][i], v[k][i], sum);
-            }
-        const float rstd = rsqrtf(row_sum(sum) * inv_c + a.eps);
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int i = 0; i < V; i++)
+                    if ((int)(k * vstep) >= left) v[k][i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            by_pairs<V>(
+                [&](int i) {
+                    const float2 z = make_float2(v[k][i], v[k][i + 1]);
+                    squares = fma2(z, z, squares);
+                },
+                [&](int) { squares.x = fmaf(v[k][0], v[k][0], squares.x); });
+        const float rstd = rsqrtf(row_sum(squares.x + squares.y) * inv_c + a.eps);
         if (live) {
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                if (k * vstep >= left) continue;
+                if ((int)(k * vstep) >= left) continue;
                 float o[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) o[i] = fmaf(v[k][i] * rstd, w[k][i], b[k][i]);
-                store_vec<T, V>(static_cast<T*>(a.y) + at + k * vstep, o);
+                by_pairs<V>(
+                    [&](int i) {
+                        const float2 z = fma2(mul2(make_float2(v[k][i], v[k][i + 1]), both(rstd)),
+                                              make_float2(w[k][i], w[k][i + 1]), make_float2(b[k][i], b[k][i + 1]));
+                        o[i] = z.x, o[i + 1] = z.y;
+                    },
+                    [&](int) { o[0] = fmaf(v[k][0] * rstd, w[k][0], b[k][0]); });
+                store_vec<T, V>(py + (at + k * vstep), o);
             }
             if (lane == 0 && a.mean) a.mean[row] = mean, a.rstd[row] = rstd;
         }
-        row += step, at += astep;
+        row += step, px += astep, py += astep;
+        if (RES) pr += astep, ps += astep;
     }
 }
 
-template <typename T, int V, int K, bool WIDE, bool RES>
-__global__ void HV_NORM_BOUNDS k_norm_backward(const NormArgs a) {
-    __shared__ float2 scratch[2][kNormMaxThreads / 32];
+template <typename T, int V, int K, int LG, bool RES>
+__global__ void HV_NORM_BOUNDS(4) k_norm_backward(const NormArgs a) {
+    constexpr bool WIDE = LG == kWide;
     __shared__ float part[WIDE ? 1 : kNormThreads * V];
-    const int G = WIDE ? blockDim.x : a.G, lane = threadIdx.x & (G - 1), groups = blockDim.x / G, group = threadIdx.x / G;
-    const int C = a.C, vstep = G * V, left = C - lane * V;
-    RowSum<WIDE> row_sum = {scratch, G, 0};
+    HV_NORM_PLACE
     float w[K][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; k++)
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            const int c = k * vstep + lane * V + i;
+            const int c = k * vstep + at + i;
             w[k][i] = c < C ? load_param<T>(a.w, c, a.w_f32) : 0.f;
             dw[k][i] = db[k][i] = 0.f;
         }
-    const float inv_c = 1.f / (float)C;
-    const int64_t step = (int64_t)gridDim.x * groups, astep = step * C;
-    int64_t row = (int64_t)blockIdx.x * groups + group, at = row * C + lane * V;
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += step) {
-        const bool live = row < a.rows;
-        RowOf<T, V, K> x, dy, ds;
-        float mean = 0.f, rstd = 0.f;
-        if (live) {
-            x.load(a.x, at, vstep, left);
-            dy.load(a.dy, at, vstep, left);
-            if (RES) ds.load(a.ds, at, vstep, left);
-            mean = a.mean[row], rstd = a.rstd[row];
-        }
-        float xh[K][V], g[K][V];
-        float2 sum = make_float2(0.f, 0.f);
+    const T *px = static_cast<const T*>(a.x) + first, *pg = static_cast<const T*>(a.dy) + first,
+            *ps = static_cast<const T*>(a.ds) + (RES ? first : 0);
+    T* pd = static_cast<T*>(a.dx) + first;
+    // Vectors past the row's end read its first values instead: their weight is
+    // zero, and their sums are not written.
+    uint32_t off[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) off[k] = (int)(k * vstep) < left ? at + k * vstep : 0;
+    struct Row {
+        Vec<T, V> x[K], dy[K], ds[K];
+        float mean, rstd;
+    };
+    auto fetch = [&](Row& r, int64_t ahead, int64_t of) {
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            const bool in = live && k * vstep < left;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                xh[k][i] = in ? (x.at(k, i) - mean) * rstd : 0.f;
-                g[k][i] = in ? dy.at(k, i) : 0.f;
-                db[k][i] += g[k][i];
-                dw[k][i] = fmaf(g[k][i], xh[k][i], dw[k][i]);
-                g[k][i] *= w[k][i];
-                sum.x += g[k][i];
-                sum.y = fmaf(g[k][i], xh[k][i], sum.y);
-            }
+            r.x[k] = *reinterpret_cast<const Vec<T, V>*>(px + ahead + off[k]);
+            r.dy[k] = *reinterpret_cast<const Vec<T, V>*>(pg + ahead + off[k]);
+            if (RES) r.ds[k] = *reinterpret_cast<const Vec<T, V>*>(ps + ahead + off[k]);
         }
-        sum = row_sum(sum);
+        r.mean = a.mean[of], r.rstd = a.rstd[of];
+    };
+    auto pair = [](const Vec<T, V>& v, int i) { return make_float2(to_f32(v.x[i]), to_f32(v.x[i + 1])); };
+    // live: this thread's group has the row r; then(): what may be loaded once r's sums are taken
+    auto turn = [&](const Row& r, bool live, auto then) {
+        const float m = r.mean, s = r.rstd;
+        float2 sg = both(0.f), sx = both(0.f);
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            by_pairs<V>(
+                [&](int i) {
+                    const float2 h = mul2(add2(pair(r.x[k], i), both(-m)), both(s)), y = pair(r.dy[k], i);
+                    const float2 e = add2(make_float2(db[k][i], db[k][i + 1]), y);
+                    const float2 f = fma2(y, h, make_float2(dw[k][i], dw[k][i + 1]));
+                    const float2 z = mul2(y, make_float2(w[k][i], w[k][i + 1]));
+                    db[k][i] = e.x, db[k][i + 1] = e.y, dw[k][i] = f.x, dw[k][i + 1] = f.y;
+                    sg = add2(sg, z), sx = fma2(z, h, sx);
+                },
+                [&](int) {
+                    const float h = (to_f32(r.x[k].x[0]) - m) * s, y = to_f32(r.dy[k].x[0]), z = y * w[k][0];
+                    db[k][0] += y;
+                    dw[k][0] = fmaf(y, h, dw[k][0]);
+                    sg.x += z;
+                    sx.x = fmaf(z, h, sx.x);
+                });
+        then();
+        const float2 sum = row_sum(make_float2(sg.x + sg.y, sx.x + sx.y));
         const float mg = sum.x * inv_c, mgx = sum.y * inv_c;
         if (live)
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                if (k * vstep >= left) continue;
+                if ((int)(k * vstep) >= left) continue;
                 float o[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    o[i] = rstd * (g[k][i] - mg - xh[k][i] * mgx);
-                    if (RES) o[i] += ds.at(k, i);
-                }
-                store_vec<T, V>(static_cast<T*>(a.dx) + at + k * vstep, o);
+                by_pairs<V>(
+                    [&](int i) {
+                        const float2 h = mul2(add2(pair(r.x[k], i), both(-m)), both(s));
+                        float2 z = fma2(pair(r.dy[k], i), make_float2(w[k][i], w[k][i + 1]), both(-mg));
+                        z = fma2(h, both(-mgx), z);
+                        z = RES ? fma2(z, both(s), pair(r.ds[k], i)) : mul2(z, both(s));
+                        o[i] = z.x, o[i + 1] = z.y;
+                    },
+                    [&](int) {
+                        const float h = (to_f32(r.x[k].x[0]) - m) * s, z = fmaf(h, -mgx, fmaf(to_f32(r.dy[k].x[0]), w[k][0], -mg));
+                        o[0] = RES ? fmaf(z, s, to_f32(r.ds[k].x[0])) : z * s;
+                    });
+                store_vec<T, V>(pd + (at + k * vstep), o);
             }
-        row += step, at += astep;
+        row += step, px += astep, pg += astep, pd += astep;
+        if (RES) ps += astep;
+    };
+    if constexpr (WIDE) {
+        // a block's one row leaves few loads in flight: the next is fetched a turn ahead
+        Row next;
+        if (r0 < a.rows) fetch(next, 0, row);
+        for (; r0 < a.rows; r0 += step) {
+            const Row r = next;
+            turn(r, true, [&] { if (r0 + step < a.rows) fetch(next, astep, row + step); });
+        }
+    } else {
+        Row r;
+        for (; r0 + groups <= a.rows; r0 += step) {
+            fetch(r, 0, row);
+            turn(r, true, [] {});
+        }
+        if (r0 < a.rows) {  // the last rows: fewer than the groups
+            const bool live = row < a.rows;
+            if (live) fetch(r, 0, row);
+            else r = {};
+            turn(r, live, [] {});
+        }
     }
     // this block's sums over its rows, in a fixed order: over the groups of a
     // warp by shuffles, over the warps through shared memory
@@ -251,7 +335,7 @@ __global__ void HV_NORM_BOUNDS k_norm_backward(const NormArgs a) {
                     for (int o = G; o < 32; o <<= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
             }
             if (WIDE) {  // one row a block: its threads own their columns
-                const int c = k * vstep + lane * V;
+                const int c = k * vstep + at;
 #pragma unroll
                 for (int i = 0; i < V; i++)
                     if (c + i < C) put(which, c + i, v[i]);
@@ -272,25 +356,30 @@ __global__ void HV_NORM_BOUNDS k_norm_backward(const NormArgs a) {
 }
 
 #undef HV_NORM_BOUNDS
+#undef HV_NORM_PLACE
 
-// Sums the blocks' partial rows [n][2][C] into dw and db: 32 columns a block,
-// 32 threads down each column.
+// Sums the blocks' partial rows [n][2][C] into dw and db in a fixed order: 8
+// columns a block, 128 threads down each.
 template <typename T>
 __global__ void __launch_bounds__(1024) k_norm_reduce(const float* __restrict__ partial, int n, int C, void* dw,
                                                       void* db, int w_f32) {
-    __shared__ float t[32][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
-    float v = 0.f;
+    __shared__ float sums[32][8];
+    const int v = threadIdx.x & 7, part = threadIdx.x >> 3, col = blockIdx.x * 8 + v;
+    float x = 0.f;
     if (col < 2 * C)
-#pragma unroll 8
-        for (int i = part; i < n; i += 32) v += partial[(int64_t)i * 2 * C + col];
-    t[part][threadIdx.x & 31] = v;
+#pragma unroll 4
+        for (int i = part; i < n; i += 128) x += partial[(int64_t)i * 2 * C + col];
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+    x += __shfl_xor_sync(0xffffffffu, x, 16);
+    if ((threadIdx.x & 31) < 8) sums[threadIdx.x >> 5][v] = x;
     __syncthreads();
-    v = t[threadIdx.x & 31][part];
+    if (threadIdx.x >= 256) return;
+    // warp c: column c's 32 sums
+    x = sums[threadIdx.x & 31][threadIdx.x >> 5];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    const int c = blockIdx.x * 32 + part;
-    if ((threadIdx.x & 31) == 0 && c < 2 * C) store_param<T>(c < C ? dw : db, c < C ? c : c - C, w_f32, v);
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    const int c = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if ((threadIdx.x & 31) == 0 && c < 2 * C) store_param<T>(c < C ? dw : db, c < C ? c : c - C, w_f32, x);
 }
 
 }  // namespace hv

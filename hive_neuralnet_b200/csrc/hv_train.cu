@@ -73,7 +73,7 @@ static int by_type(int dtype, F f) {
 // ---------------------------------------------------------------------------
 // layer norm
 // ---------------------------------------------------------------------------
-constexpr int kNormMaxWidth = kNormMaxThreads * kNormValues;
+constexpr int kNormMaxWidth = kNormMaxThreads * kNormValuesWide;
 constexpr int kNormBlocksPerSm = 8;  // at most
 
 struct NormShape {
@@ -83,23 +83,19 @@ struct NormShape {
 
 // V values a vector where rows and pointers allow 16-byte vectors, else 1.  A
 // row goes to the fewest threads of a warp that hold it at 8 values each (the
-// more values a thread, the fewer shuffles a value), or to a block.
+// more values a thread, the fewer shuffles a value), or to a block, at 8 values
+// a thread up to 4096, 16 up to 8192.
 static bool norm_shape(int C, int dtype, bool vec, NormShape* s) {
     s->V = vec ? (int)(16 / elem_bytes(dtype)) : 1;
     const int n = (C + s->V - 1) / s->V;  // vectors of a row
-    s->wide = C > 32 * kNormValuesWarp;
-    if (s->wide) {
-        s->threads = 128;
-        while (s->threads < kNormMaxThreads && n * s->V > s->threads * (kNormValues / 2)) s->threads *= 2;
-        s->G = s->threads;
-    } else {
-        s->threads = kNormThreads;
-        s->G = 1;
-        while (n * s->V > s->G * kNormValuesWarp) s->G *= 2;
-    }
+    s->wide = C > 32 * kNormValues;
+    s->threads = s->wide ? 128 : kNormThreads;
+    while (s->wide && s->threads < kNormMaxThreads && n * s->V > s->threads * kNormValues) s->threads *= 2;
+    s->G = s->wide ? s->threads : 1;
+    while (!s->wide && n * s->V > s->G * kNormValues) s->G *= 2;
     s->K = 1;
     while (s->K * s->G < n) s->K *= 2;
-    return s->K * s->V <= (s->wide ? kNormValues : kNormValuesWarp);
+    return s->K * s->V <= (s->wide ? kNormValuesWide : kNormValues);
 }
 
 static bool norm_vec(int C, int dtype, std::initializer_list<const void*> ptrs) {
@@ -128,25 +124,38 @@ static int launch_norm(const NormArgs& a, const NormShape& s, int* grid, cudaStr
         kernel<<<*grid, s.threads, 0, st>>>(a);
         return launched();
     };
-    constexpr int V = 16 / sizeof(T);
-#define HV_NORM(VV, KK, WW)                                                    \
-    if constexpr (VV * KK <= (WW ? kNormValues : kNormValuesWarp))             \
-        if (s.V == VV && s.K == KK && s.wide == WW) {                          \
-            if constexpr (BACK) return go(k_norm_backward<T, VV, KK, WW, RES>); \
-            else return go(k_norm_forward<T, VV, KK, WW, RES>);                \
+    constexpr int V = 16 / sizeof(T), KV = kNormValues / V;  // a row within a warp: KV vectors a thread (narrower: one)
+#define HV_NORM(VV, KK, LL)                                                 \
+    if constexpr (BACK) return go(k_norm_backward<T, VV, KK, LL, RES>);     \
+    else return go(k_norm_forward<T, VV, KK, LL, RES>);
+    if (s.wide) {
+        if (s.V == 1) {
+            if (s.K == 4) { HV_NORM(1, 4, kWide) }
+            if (s.K == 8) { HV_NORM(1, 8, kWide) }
+            if (s.K == 16) { HV_NORM(1, 16, kWide) }
+        } else {
+            if (s.K == 1) { HV_NORM(V, 1, kWide) }
+            if (s.K == 2) { HV_NORM(V, 2, kWide) }
+            if constexpr (V == 4)
+                if (s.K == 4) { HV_NORM(V, 4, kWide) }
         }
-    HV_NORM(V, 1, false)
-    HV_NORM(V, 2, false)
-    HV_NORM(1, 1, false)
-    HV_NORM(1, 2, false)
-    HV_NORM(1, 4, false)
-    HV_NORM(1, 8, false)
-    HV_NORM(V, 1, true)
-    HV_NORM(V, 2, true)
-    HV_NORM(V, 4, true)
-    HV_NORM(1, 4, true)
-    HV_NORM(1, 8, true)
-    HV_NORM(1, 16, true)
+    } else if (s.V == 1) {
+        if (s.K == 1) { HV_NORM(1, 1, kLoose) }
+        if (s.K == 2) { HV_NORM(1, 2, kLoose) }
+        if (s.K == 4) { HV_NORM(1, 4, kLoose) }
+        if (s.K == 8) { HV_NORM(1, 8, kLoose) }
+    } else if (s.K < KV) {
+        if constexpr (KV > 1) { HV_NORM(V, 1, 0) }
+    } else {
+        switch (s.G) {
+            case 1: HV_NORM(V, KV, 0)
+            case 2: HV_NORM(V, KV, 1)
+            case 4: HV_NORM(V, KV, 2)
+            case 8: HV_NORM(V, KV, 3)
+            case 16: HV_NORM(V, KV, 4)
+            case 32: HV_NORM(V, KV, 5)
+        }
+    }
 #undef HV_NORM
     return HV_EINVAL;
 }
@@ -412,7 +421,7 @@ int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, co
             const int rc = dsum ? launch_norm<T, true, true>(a, s, &grid, st) : launch_norm<T, true, false>(a, s, &grid, st);
             if (rc || grid == 1) return rc;
         }
-        k_norm_reduce<T><<<(2 * width + 31) / 32, 1024, 0, st>>>(a.partial, grid, width, dweight, dbias, a.w_f32);
+        k_norm_reduce<T><<<(2 * width + 7) / 8, 1024, 0, st>>>(a.partial, grid, width, dweight, dbias, a.w_f32);
         return launched();
     });
 }
