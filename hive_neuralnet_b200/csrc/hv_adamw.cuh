@@ -3,8 +3,8 @@
 //   m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// Every product and sum is rounded by itself (no contraction), so a step is
-// the same on every path.  The moments live in two flat arrays; a tensor's
+// Every product and sum of the moments is rounded by itself (no contraction):
+// they are the same on every path, to the bit.  The moments live in two flat arrays; a tensor's
 // part begins at a multiple of 256 values.
 //
 // 8-bit moments: a scale for each 256 values (largest magnitude / largest
@@ -50,8 +50,7 @@ __device__ __forceinline__ uint32_t adam_hash(uint64_t i, uint32_t key) {
 }
 
 __device__ __forceinline__ float code_value_m(uint32_t c) {
-    const float y = __uint_as_float((c & 127u) << 20) * 0x1p120f;
-    return c & 128u ? -y : y;
+    return __uint_as_float((c & 128u) << 24 | (c & 127u) << 20) * 0x1p120f;
 }
 
 __device__ __forceinline__ float code_value_r(uint32_t c) { return __uint_as_float(c << 19) * 0x1p120f; }
@@ -61,143 +60,209 @@ __device__ __forceinline__ uint32_t encode(float y, uint32_t noise, int shift, u
     return c < top ? c : top;
 }
 
-__device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v, const AdamScalars& s) {
+// root: sqrt of the new v.  The quotient alone is approximate (2 ulps): it only
+// reaches p, of which it is a small part.
+__device__ __forceinline__ void adam_value(float& p, float g, float& m, float& v, float& root, const AdamScalars& s) {
     m = __fadd_rn(__fmul_rn(m, s.b1), __fmul_rn(g, s.one_b1));
     v = __fadd_rn(__fmul_rn(v, s.b2), __fmul_rn(__fmul_rn(g, g), s.one_b2));
-    const float denom = __fadd_rn(__fmul_rn(__fsqrt_rn(v), s.inv_root_bc2), s.eps);
-    p = __fsub_rn(__fmul_rn(p, s.decay), __fmul_rn(__fdiv_rn(m, denom), s.step_size));
+    root = __fsqrt_rn(v);
+    const float denom = __fadd_rn(__fmul_rn(root, s.inv_root_bc2), s.eps);
+    p = __fsub_rn(__fmul_rn(p, s.decay), __fmul_rn(__fmul_rn(m, rcp_approx(denom)), s.step_size));
 }
 
-// 4 values at p + i of a tensor of n values; whole vectors where they fit.
+// A tensor of a launch's table, and the 256-value unit of it that a warp takes.
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t i, int64_t n, bool vec, float* x) {
-    if (vec && i + 4 <= n) {
-        load_vec<T, 4>(p + i, x);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = i + j < n ? to_f32(p[i + j]) : 0.f;
-    }
-}
+struct AdamUnit {
+    T* p;
+    const T* g;
+    int64_t n, at;  // values of the tensor; the unit's first
+    bool vec;
 
+    // the tensor of a unit is sought from tensor `from` on (its first unit is not above the unit)
+    template <int CAP>
+    __device__ __forceinline__ int find(const AdamTable<CAP>& t, int unit, int from) {
+        int lo = from, hi = t.tensors;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (t.first[mid] <= unit)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        p = static_cast<T*>(t.p[lo]);
+        g = static_cast<const T*>(t.g[lo]);
+        n = t.n[lo], at = (int64_t)(unit - t.first[lo]) * kAdamBlock;
+        vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(T) - 1)) == 0 &&
+              at + kAdamBlock <= n;
+        return lo;
+    }
+};
+
+// A lane's 4 + 4 values of a unit as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int64_t i, int64_t n, bool vec, const float* x) {
-    if (vec && i + 4 <= n) {
-        store_vec<T, 4>(p + i, x);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (i + j < n) p[i + j] = from_f32<T>(x[j]);
-    }
-}
-
-// One warp takes 256 values, 4 + 4 a lane.  unit0: the table's first unit in
-// the flat states.
-template <typename T, bool SMALL, int CAP>
-__global__ void __launch_bounds__(kAdamWarps * 32) k_adamw(const __grid_constant__ AdamTable<CAP> t, void* m_all,
-                                                           void* v_all, float* m_scale, float* v_scale,
-                                                           int64_t unit0, const AdamScalars s) {
-    const int unit = blockIdx.x * kAdamWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (unit >= t.first[t.tensors]) return;
-    int lo = 0, hi = t.tensors;  // the last tensor whose first unit is <= unit
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (t.first[mid] <= unit)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    T* p = static_cast<T*>(t.p[lo]);
-    const T* g = static_cast<const T*>(t.g[lo]);
-    const int64_t n = t.n[lo], at = (int64_t)(unit - t.first[lo]) * kAdamBlock;
-    const bool vec = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & (4 * sizeof(T) - 1)) == 0;
-    const int64_t u = unit0 + unit, flat = u * kAdamBlock;
-    float P[8], M[8], R[8], Gr[8];
+__device__ __forceinline__ void load8(const T* p, int64_t at, int64_t n, bool vec, int lane, Vec<T, 4> (&x)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        load4<T>(p, at + h * 128 + lane * 4, n, vec, P + h * 4);
-        load4<T>(g, at + h * 128 + lane * 4, n, vec, Gr + h * 4);
+        const int64_t i = at + h * 128 + lane * 4;
+        if (vec) {
+            x[h] = *reinterpret_cast<const Vec<T, 4>*>(p + i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[h].x[j] = i + j < n ? p[i + j] : from_f32<T>(0.f);
+        }
     }
-    if (!SMALL) {
-        float* m = static_cast<float*>(m_all) + flat;
-        float* v = static_cast<float*>(v_all) + flat;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t at, int64_t n, bool vec, int lane, const float* x) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            load_vec<float, 4>(m + h * 128 + lane * 4, M + h * 4);
-            load_vec<float, 4>(v + h * 128 + lane * 4, R + h * 4);
+    for (int h = 0; h < 2; h++) {
+        const int64_t i = at + h * 128 + lane * 4;
+        if (vec) {
+            store_vec<T, 4>(p + i, x + 4 * h);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < n) p[i + j] = from_f32<T>(x[4 * h + j]);
         }
+    }
+}
+
+// fp32 states.  unit0: the table's first unit in the flat states.
+template <typename T, int CAP>
+__global__ void __launch_bounds__(kAdamWarps * 32) k_adamw(const __grid_constant__ AdamTable<CAP> t, float* m_all,
+                                                           float* v_all, int64_t unit0, const AdamScalars s) {
+    const int unit = blockIdx.x * kAdamWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (unit >= t.first[t.tensors]) return;
+    AdamUnit<T> u;
+    u.find(t, unit, 0);
+    float* m = m_all + (unit0 + unit) * kAdamBlock + lane * 4;
+    float* v = v_all + (unit0 + unit) * kAdamBlock + lane * 4;
+    Vec<T, 4> p4[2], g4[2];
+    float P[8], M[8], R[8], root;
+    load8(u.p, u.at, u.n, u.vec, lane, p4);
+    load8(u.g, u.at, u.n, u.vec, lane, g4);
 #pragma unroll
-        for (int i = 0; i < 8; i++) adam_value(P[i], Gr[i], M[i], R[i], s);
+    for (int h = 0; h < 2; h++) {
+        load_vec<float, 4>(m + h * 128, M + h * 4);
+        load_vec<float, 4>(v + h * 128, R + h * 4);
+    }
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            store_vec<float, 4>(m + h * 128 + lane * 4, M + h * 4);
-            store_vec<float, 4>(v + h * 128 + lane * 4, R + h * 4);
+    for (int i = 0; i < 8; i++) {
+        P[i] = to_f32(p4[i >> 2].x[i & 3]);
+        adam_value(P[i], to_f32(g4[i >> 2].x[i & 3]), M[i], R[i], root, s);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        store_vec<float, 4>(m + h * 128, M + h * 4);
+        store_vec<float, 4>(v + h * 128, R + h * 4);
+    }
+    store8(u.p, u.at, u.n, u.vec, lane, P);
+}
+
+// 8-bit states.  A warp takes every gridDim.x * kAdamWarps-th unit and loads the
+// next while it computes one: decoding, rounding and encoding are about 100
+// instructions a value, and with one unit a warp each waited for its loads.
+template <typename T, int CAP>
+__global__ void __launch_bounds__(kAdamWarps * 32, 3) k_adamw8(const __grid_constant__ AdamTable<CAP> t, uint32_t* m_all,
+                                                               uint32_t* v_all, float* m_scale, float* v_scale,
+                                                               int64_t unit0, const AdamScalars s) {
+    struct Loaded {
+        Vec<T, 4> p[2], g[2];
+        uint32_t m[2], v[2];
+        float ms, vs;
+    };
+    const int lane = threadIdx.x & 31, units = t.first[t.tensors], step = gridDim.x * kAdamWarps;
+    AdamUnit<T> u, ahead = {};
+    Loaded next;
+    auto fetch = [&](int unit) {
+        load8(ahead.p, ahead.at, ahead.n, ahead.vec, lane, next.p);
+        load8(ahead.g, ahead.at, ahead.n, ahead.vec, lane, next.g);
+        const int64_t w = (unit0 + unit) * (kAdamBlock / 4) + lane;
+#pragma unroll
+        for (int h = 0; h < 2; h++) next.m[h] = m_all[w + h * 32], next.v[h] = v_all[w + h * 32];
+        next.ms = m_scale[unit0 + unit], next.vs = v_scale[unit0 + unit];
+    };
+    int unit = blockIdx.x * kAdamWarps + (threadIdx.x >> 5), tensor = 0;
+    if (unit < units) {
+        tensor = ahead.find(t, unit, 0);
+        fetch(unit);
+    }
+    for (; unit < units; unit += step) {
+        const Loaded x = next;
+        u = ahead;
+        if (unit + step < units) {
+            tensor = ahead.find(t, unit + step, tensor);
+            fetch(unit + step);
         }
-    } else {
-        uint32_t* mc = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(m_all) + flat);
-        uint32_t* vc = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(v_all) + flat);
-        const float ms = m_scale[u], vs = v_scale[u];
-        float top_m = 0.f, top_r = 0.f;
+        float P[8], M[8], R[8], top_m = 0.f, top_r = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const uint32_t a = mc[h * 32 + lane], b = vc[h * 32 + lane];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int i = h * 4 + j;
-                M[i] = __fmul_rn(code_value_m((a >> (8 * j)) & 255u), ms);
-                const float r = __fmul_rn(code_value_r((b >> (8 * j)) & 255u), vs);
-                R[i] = __fmul_rn(r, r);
-                adam_value(P[i], Gr[i], M[i], R[i], s);
-                R[i] = __fsqrt_rn(R[i]);
-                top_m = fmaxf(top_m, fabsf(M[i]));
-                top_r = fmaxf(top_r, R[i]);
-            }
+        for (int i = 0; i < 8; i++) {
+            const int h = i >> 2, j = i & 3;
+            M[i] = __fmul_rn(code_value_m((x.m[h] >> (8 * j)) & 255u), x.ms);
+            const float r = __fmul_rn(code_value_r((x.v[h] >> (8 * j)) & 255u), x.vs);
+            float v = __fmul_rn(r, r);
+            P[i] = to_f32(x.p[h].x[j]);
+            adam_value(P[i], to_f32(x.g[h].x[j]), M[i], v, R[i], s);
+            top_m = fmaxf(top_m, fabsf(M[i]));
+            top_r = fmaxf(top_r, R[i]);
         }
+        store8(u.p, u.at, u.n, u.vec, lane, P);
         // non-negative floats order as their bits do
         top_m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)));
         top_r = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_r)));
         const bool live_m = top_m >= 0x1p-100f, live_r = top_r >= 0x1p-100f;  // below: no scale is kept
         const float inv_m = __fdiv_rn(kCodeMaxM, top_m), inv_r = __fdiv_rn(kCodeMaxR, top_r);
+        const uint64_t flat = (uint64_t)(unit0 + unit) * kAdamBlock + lane * 4;
+        const int64_t w = (unit0 + unit) * (kAdamBlock / 4) + lane;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             uint32_t a = 0, b = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int i = h * 4 + j;
-                const uint32_t noise = adam_hash((uint64_t)(flat + h * 128 + lane * 4 + j), s.key);
+                const uint32_t noise = adam_hash(flat + h * 128 + j, s.key);
                 uint32_t c = encode(__fmul_rn(fabsf(M[i]), inv_m), noise & 0xFFFFFu, 20, 127u) | (M[i] < 0.f ? 128u : 0u);
-                a |= (live_m ? c : 0u) << (8 * j);
+                a |= c << (8 * j);
                 c = encode(__fmul_rn(R[i], inv_r), noise >> 13, 19, 255u);
                 c = R[i] > 0.f && c == 0u ? 1u : c;
-                b |= (live_r ? c : 0u) << (8 * j);
+                b |= c << (8 * j);
             }
-            mc[h * 32 + lane] = a;
-            vc[h * 32 + lane] = b;
+            m_all[w + h * 32] = live_m ? a : 0u;
+            v_all[w + h * 32] = live_r ? b : 0u;
         }
-        if (lane == 0) {
-            m_scale[u] = live_m ? __fdiv_rn(top_m, kCodeMaxM) : 0.f;
-            v_scale[u] = live_r ? __fdiv_rn(top_r, kCodeMaxR) : 0.f;
+        if (lane < 2) {
+            const float scale = lane ? __fdiv_rn(top_r, kCodeMaxR) : __fdiv_rn(top_m, kCodeMaxM);
+            (lane ? v_scale : m_scale)[unit0 + unit] = (lane ? live_r : live_m) ? scale : 0.f;
         }
     }
-#pragma unroll
-    for (int h = 0; h < 2; h++) store4<T>(p, at + h * 128 + lane * 4, n, vec, P + h * 4);
 }
 
-// The values that 8-bit states stand for, 4 a thread.
+// The values that 8-bit states stand for, 4 x 4 a thread.
 template <bool SECOND>
 __global__ void __launch_bounds__(256) k_adamw_values(const uint32_t* __restrict__ codes,
                                                       const float* __restrict__ scale, int64_t words, float* out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= words) return;
-    const uint32_t c = codes[i];
-    const float s = scale[i / (kAdamBlock / 4)];
-    float x[4];
+    const int64_t i0 = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+    uint32_t c[4];
+    float s[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t b = (c >> (8 * j)) & 255u;
-        x[j] = __fmul_rn(SECOND ? code_value_r(b) : code_value_m(b), s);
-        if (SECOND) x[j] = __fmul_rn(x[j], x[j]);
+    for (int k = 0; k < 4; k++) {
+        const int64_t i = i0 + k * 256;
+        if (i < words) c[k] = codes[i], s[k] = scale[i / (kAdamBlock / 4)];
     }
-    store_vec<float, 4>(out + i * 4, x);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int64_t i = i0 + k * 256;
+        if (i >= words) break;
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t b = (c[k] >> (8 * j)) & 255u;
+            x[j] = __fmul_rn(SECOND ? code_value_r(b) : code_value_m(b), s[k]);
+            if (SECOND) x[j] = __fmul_rn(x[j], x[j]);
+        }
+        store_vec<float, 4>(out + i * 4, x);
+    }
 }
 
 }  // namespace hv

@@ -65,6 +65,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return d;
 }
 
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // A value of a small fp32-or-T parameter tensor (weights, bias tables).
 template <typename T>
 __device__ __forceinline__ float load_param(const void* p, int64_t i, bool is_f32) {

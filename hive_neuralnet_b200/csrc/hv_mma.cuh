@@ -317,10 +317,4 @@ __device__ __forceinline__ void add_at(uint32_t p, uint32_t q, uint32_t r, float
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(r), "f"(c));
 }
 
-__device__ __forceinline__ float rcp_approx(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 }  // namespace hv

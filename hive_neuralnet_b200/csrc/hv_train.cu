@@ -461,13 +461,18 @@ int hv_adamw_step(void* const* params, const void* const* grads, const int64_t* 
             }
             if (!n) break;
             tab.first[n] = (int32_t)units, tab.tensors = n;
-            const unsigned grid = (unsigned)((units + kAdamWarps - 1) / kAdamWarps);
-            if (small)
-                k_adamw<T, true, CAP><<<grid, kAdamWarps * 32, 0, (cudaStream_t)stream>>>(tab, exp_avg, exp_avg_sq, avg_scale,
-                                                                                         sq_scale, unit0, sc);
-            else
-                k_adamw<T, false, CAP><<<grid, kAdamWarps * 32, 0, (cudaStream_t)stream>>>(tab, exp_avg, exp_avg_sq, nullptr,
-                                                                                          nullptr, unit0, sc);
+            const int64_t blocks = (units + kAdamWarps - 1) / kAdamWarps;
+            if (small) {
+                int resident = 0;
+                const int rc = resident_blocks(k_adamw8<T, CAP>, kAdamWarps * 32, 0, &resident);
+                if (rc) return rc;
+                const int64_t most = (int64_t)sm_count() * resident;
+                k_adamw8<T, CAP><<<(unsigned)(blocks < most ? blocks : most), kAdamWarps * 32, 0, (cudaStream_t)stream>>>(
+                    tab, static_cast<uint32_t*>(exp_avg), static_cast<uint32_t*>(exp_avg_sq), avg_scale, sq_scale, unit0, sc);
+            } else {
+                k_adamw<T, CAP><<<(unsigned)blocks, kAdamWarps * 32, 0, (cudaStream_t)stream>>>(
+                    tab, static_cast<float*>(exp_avg), static_cast<float*>(exp_avg_sq), unit0, sc);
+            }
             const int rc = launched();
             if (rc) return rc;
             unit0 += units;
@@ -483,7 +488,7 @@ int hv_adamw_state_values(const uint8_t* codes, const float* scale, int64_t coun
     if (count < 0 || count % kAdamBlock) return HV_EINVAL;
     if (count == 0) return HV_OK;
     if (!codes || !scale || !out || !aligned(codes, 4) || !aligned(out, 16)) return HV_EINVAL;
-    const int64_t words = count / 4, grid = (words + 255) / 256;
+    const int64_t words = count / 4, grid = (words + 1023) / 1024;
     if (grid > 0x7fffffff) return HV_EINVAL;
     const uint32_t* c = reinterpret_cast<const uint32_t*>(codes);
     if (second)
