@@ -37,6 +37,26 @@ struct AttnArgs {
 
 __device__ __forceinline__ int coord(int x) { return min(max(x, -kCoordMax), kCoordMax); }
 
+// A pair's classes, times 4: from 4 x the key's coordinates and 4 x (clip less
+// the query's).
+struct Classes {
+    int top, top_z, W, q, r, z;
+    __device__ explicit Classes(const AttnArgs& a) : top(8 * a.clip), top_z(8 * a.clip_z), W(2 * a.clip + 1), q(0), r(0), z(0) {}
+    __device__ __forceinline__ void of(int kq, int kr, int kz, int qq, int qr, int qz) {
+        q = __viaddmin_s32_relu(kq, qq, top), r = __viaddmin_s32_relu(kr, qr, top), z = __viaddmin_s32_relu(kz, qz, top_z);
+    }
+};
+
+// The bias in two terms: dz and dq from one table [dz][dq], dr from another
+// (one lookup less than three tables; all three joined would be 1445 entries a
+// head, to be built by every block, with bank conflicts at every lookup).
+__device__ __forceinline__ float2 bias_of(const char* joined, const char* dr, const Classes& c) {
+    return make_float2(*reinterpret_cast<const float*>(joined + (c.z * c.W + c.q)), *reinterpret_cast<const float*>(dr + c.r));
+}
+
+// A value that all lanes of a warp have, as one that the compiler knows to be so.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // Sums n partial tables [n][classes][H] in a fixed order: a block takes 8
 // values, 128 threads down each.
 template <typename T>

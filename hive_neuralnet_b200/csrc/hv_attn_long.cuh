@@ -114,22 +114,6 @@ __device__ __forceinline__ void load_bias_table(char* smem, const AttnArgs& a, i
     }
 }
 
-// A pair's classes, times 4: from 4 x the key's coordinates and 4 x (clip less
-// the query's).
-struct Classes {
-    int top, top_z, W, q, r, z;
-    __device__ explicit Classes(const AttnArgs& a) : top(8 * a.clip), top_z(8 * a.clip_z), W(2 * a.clip + 1), q(0), r(0), z(0) {}
-    __device__ __forceinline__ void of(int kq, int kr, int kz, int qq, int qr, int qz) {
-        q = __viaddmin_s32_relu(kq, qq, top), r = __viaddmin_s32_relu(kr, qr, top), z = __viaddmin_s32_relu(kz, qz, top_z);
-    }
-};
-
-// The bias, in two terms.
-__device__ __forceinline__ float2 bias_of(const char* smem, const Classes& c) {
-    return make_float2(*reinterpret_cast<const float*>(smem + (c.z * c.W + c.q)),
-                       *reinterpret_cast<const float*>(smem + c.r + kTabR * 4));
-}
-
 // BACK false: the forward pass; true: dq (and delta).  A warp takes 16 of the
 // ROWS queries and 1 / WK of each tile's keys.
 template <typename T, int DP, int ROWS, int WK, bool BACK>
@@ -263,9 +247,9 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 cls.of(ma.x, ma.y, ma.z, qq[r], qr[r], qz[r]);
-                const float2 ba = bias_of(smem, cls);
+                const float2 ba = bias_of(smem, smem + kTabR * 4, cls);
                 cls.of(mb.x, mb.y, mb.z, qq[r], qr[r], qz[r]);
-                const float2 bb = bias_of(smem, cls);
+                const float2 bb = bias_of(smem, smem + kTabR * 4, cls);
                 const float2 x = fma2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(scale2, scale2),
                                       add2(make_float2(ba.x, bb.x), make_float2(ba.y, bb.y)));
                 s[j][2 * r] = x.x, s[j][2 * r + 1] = x.y;
@@ -537,7 +521,7 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
                     Classes ca = cls, cb = cls;
                     ca.of(kq[r], kr[r], kz[r], -ma.x, -ma.y, -ma.z);
                     cb.of(kq[r], kr[r], kz[r], -mb.x, -mb.y, -mb.z);
-                    const float2 ba = bias_of(smem, ca), bb = bias_of(smem, cb);
+                    const float2 ba = bias_of(smem, smem + kTabR * 4, ca), bb = bias_of(smem, smem + kTabR * 4, cb);
                     float2 y2 = fma2(make_float2(s[j][2 * r], s[j][2 * r + 1]), make_float2(scale2, scale2),
                                      add2(make_float2(ba.x, bb.x), make_float2(ba.y, bb.y)));
                     y2 = add2(y2, make_float2(-x.x, -x.z));

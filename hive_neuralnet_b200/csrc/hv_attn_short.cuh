@@ -1,17 +1,20 @@
 // hv_attn_short.cuh -- the attention of hv_attn.cuh for up to 32 tokens, the
 // network's own case (28 piece tokens and CLS).
 //
-// A block takes one position and a group of heads at a time, a warp one head:
-// the position's rows come into shared memory once, coalesced over the heads,
-// while the position before is computed.  Masked tokens are left out when the
+// A warp takes one head and walks over positions by itself: it copies its
+// head's rows into its own shared memory while it computes the position
+// before, and meets no other warp.  (With the rows of all heads copied
+// together by a block, whole lines at a time, the three barriers a position
+// cost more than the copies saved.)  The warps of a block take neighbouring
+// heads, whose rows share sectors in L1.  Masked tokens are left out when the
 // rows are stored, so a position costs what its valid tokens cost (an opening
 // position has a few of its 28).  A head's scores (two 16 x 32 tiles at most)
 // stay in registers from the first product to the last; the backward pass
 // recomputes them from q and k, so nothing is kept between the passes.
-// Results overwrite the operands they no longer need and leave in whole rows.
+// Results overwrite the operands they no longer need and leave row by row.
 //
 // Bias-table gradients: every lane adds into its own column of a [class][lane]
-// table in shared memory for all positions its block takes; the columns are
+// table in shared memory for all positions its warp takes; the columns are
 // summed once at the end, in a fixed order.
 #pragma once
 
@@ -23,85 +26,41 @@ namespace hv {
 constexpr int kSlots = 32;  // tokens of a position after compaction
 
 struct ShortPlan {
-    int HG, groups;            // heads a block, groups of heads
+    int HG, groups;            // heads (warps) a block, groups of heads
     int row;                   // bytes of a row of one operand in shared memory
-    int stage, tables, total;  // bytes: one stage, the tables before the stages, all
+    int stage, warp, total;    // bytes: one stage of a warp, a warp's part, all
     int vec_in, vec_out;       // 16-byte copies
     int per_group;             // blocks for each group of heads
 };
 
-// The copies between global memory and the slots.  A unit is half the rows
-// (16) of one operand, and a warp's: 16-byte pieces, each lane at its own
-// place in a row, 32 / pieces rows at a time.
-template <typename T, int DP>
-struct RowCopy {
-    int D, row, width;
-    bool vec;
-    int r0, rows, at, lane, head, piece;  // 16-byte pieces: the lane's first row, rows at a time, its bytes in a slot
+__device__ __forceinline__ int slot_of(uint32_t valid, int r) { return __popc(valid & ((1u << r) - 1)); }
 
-    __device__ void init(int heads, int D_, int row_, bool vec_) {
-        D = D_, row = row_, vec = vec_, width = heads * D_, lane = threadIdx.x & 31;
-        const int per_head = D * (int)sizeof(T) / 16, pieces = heads * per_head;
-        if (vec) {
-            rows = 32 / pieces, r0 = lane / pieces;
-            const int x = lane - r0 * pieces;
-            head = x / per_head, piece = x - head * per_head;
-            at = head * DP * (int)sizeof(T) + piece * 16;
-            if (r0 >= rows) r0 = kSlots;  // lanes past the last whole row
-        }
+// A head's rows between global memory and a warp's slots value by value: any
+// strides, sizes and alignment.
+template <typename T>
+__device__ __forceinline__ void load_rows(char* dst, int row, const T* src, int64_t stride, int n, int D, uint32_t valid) {
+    for (int i = threadIdx.x & 31; i < n * D; i += 32) {
+        const int r = i / D, d = i - r * D;
+        if (valid >> r & 1) reinterpret_cast<T*>(dst + slot_of(valid, r) * row)[d] = src[r * stride + d];
     }
-    __device__ static int slot(uint32_t valid, int r) { return __popc(valid & ((1u << r) - 1)); }
+}
 
-    // half 0, 1: rows 16 half .. of the n tokens
-    __device__ void load(char* dst, const void* src, const int64_t* s, int64_t b, int h0, int n, int half,
-                         uint32_t valid) const {
-        const T* base = static_cast<const T*>(src) + b * s[0] + h0 * s[2];
-        const int end = min(n, 16 * half + 16);
-        if (vec) {
-            const T* p = base + head * s[2] + piece * (16 / (int)sizeof(T));
-            for (int r = 16 * half + r0; r < end; r += rows)
-                if (valid >> r & 1) cp_async16(dst + slot(valid, r) * row + at, p + r * s[1]);
-        } else {
-            for (int i = 16 * half * width + lane; i < end * width; i += 32) {
-                const int r = i / width, c = i - r * width, h = c / D, d = c - h * D;
-                if (valid >> r & 1)
-                    reinterpret_cast<T*>(dst + slot(valid, r) * row)[h * DP + d] = base[r * s[1] + h * s[2] + d];
-            }
-        }
-        if (half == 0) {  // the slots up to the next multiple of 16 count as zero rows
-            const int c = __popc(valid & (n < 32 ? (1u << n) - 1 : 0xffffffffu));
-            uint4* z = reinterpret_cast<uint4*>(dst + c * row);
-            for (int i = lane; i < (-c & 15) * (row >> 4); i += 32) z[i] = make_uint4(0, 0, 0, 0);
-        }
+template <typename T>
+__device__ __forceinline__ void store_rows(const char* src, int row, T* dst, int64_t stride, int n, int D, uint32_t valid) {
+    for (int i = threadIdx.x & 31; i < n * D; i += 32) {
+        const int r = i / D, d = i - r * D;
+        dst[r * stride + d] = valid >> r & 1 ? reinterpret_cast<const T*>(src + slot_of(valid, r) * row)[d] : from_f32<T>(0.f);
     }
-    __device__ void store(const char* src, void* dst, const int64_t* s, int64_t b, int h0, int n, int half,
-                          uint32_t valid) const {
-        T* base = static_cast<T*>(dst) + b * s[0] + h0 * s[2];
-        const int end = min(n, 16 * half + 16);
-        if (vec) {
-            T* p = base + head * s[2] + piece * (16 / (int)sizeof(T));
-            for (int r = 16 * half + r0; r < end; r += rows) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (valid >> r & 1) v = *reinterpret_cast<const uint4*>(src + slot(valid, r) * row + at);
-                *reinterpret_cast<uint4*>(p + r * s[1]) = v;
-            }
-        } else {
-            for (int i = 16 * half * width + lane; i < end * width; i += 32) {
-                const int r = i / width, c = i - r * width, h = c / D, d = c - h * D;
-                T v = from_f32<T>(0.f);
-                if (valid >> r & 1) v = reinterpret_cast<const T*>(src + slot(valid, r) * row)[h * DP + d];
-                base[r * s[1] + h * s[2] + d] = v;
-            }
-        }
-    }
-};
+}
 
-// Byte offsets (4 x class) of a pair's three classes; the coordinates are
-// multiplied by 4 and the query's are negated with 4 clip added.
-struct ClassOf {
-    int top, top_z;
-    __device__ __forceinline__ int q(int key, int query) const { return __viaddmin_s32_relu(key, query, top); }
-    __device__ __forceinline__ int z(int key, int query) const { return __viaddmin_s32_relu(key, query, top_z); }
+// A lane's pointer into an operand's rows, moved on from position to position.
+struct Walk {
+    char* at;
+    int64_t turn, pass;  // bytes from one position of this warp to its next, from one pass over the rows to the next
+    __device__ void init(const void* base, const int64_t* s, int64_t b, int64_t step, int head, int row, int rows, int byte, int e) {
+        at = static_cast<char*>(const_cast<void*>(base)) + (b * s[0] + head * s[2] + row * s[1]) * e + byte;
+        turn = step * s[0] * e, pass = rows * s[1] * e;
+    }
 };
 
 template <typename T, int DP, bool BACK>
@@ -110,99 +69,139 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
     constexpr int NC = DP / 8, CB = NC < 4 ? NC : 4, PARTS = kParts<T>;  // 8-value chunks of a head
     constexpr bool F32 = sizeof(T) == 4;
     extern __shared__ __align__(16) char smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
-    const int group = blockIdx.x % p.groups, h0 = group * p.HG, heads = min(p.HG, a.H - h0);
+    const int lane = threadIdx.x & 31, warp = uniform(threadIdx.x >> 5), g = lane >> 2, t = lane & 3;
+    const int head = blockIdx.x % p.groups * p.HG + warp;
+    if (head >= a.H) return;  // no warp waits for another
     const int W = 2 * a.clip + 1, Z = 2 * a.clip_z + 1, classes = 2 * W + Z;
-    const int ld = p.row / (int)sizeof(T);
+    const int ld = p.row / (int)sizeof(T), operand = kSlots * p.row;
     constexpr float kLog2e = 1.4426950408889634f;
 
-    // the transposes' room (float2 words: first, where it is aligned), bias
-    // (times log2 e) [head][class], the lanes' sums
-    float* scratch = reinterpret_cast<float*>(smem);
-    float* tab = scratch + (BACK && F32 ? p.HG * 16 * kTransposeLd : 0);
-    float* hist = tab + p.HG * classes;
-    char* stages = smem + p.tables;
-    for (int i = threadIdx.x; i < p.HG * classes; i += blockDim.x) {
-        const int h = i / classes, c = i - h * classes;
-        float v = 0.f;
-        if (h < heads) {
-            const void* src = c < W ? a.bq : c < 2 * W ? a.br : a.bz;
-            v = load_param<T>(src, (int64_t)(c < W ? c : c < 2 * W ? c - W : c - 2 * W) * a.H + h0 + h, a.t_f32);
-        }
+    // a warp's part: two stages, the transposes' room, the bias (times log2 e)
+    // [dz][dq, dz joined; then dr], the lanes' sums
+    char* stages = smem + warp * p.warp;
+    float* room = reinterpret_cast<float*>(stages + 2 * p.stage);
+    float* tab = room + (BACK && F32 ? 16 * kTransposeLd : 0);
+    float* hist = tab + (Z + 1) * W;
+    for (int i = lane; i < (Z + 1) * W; i += 32) {
+        const int z = i / W, c = i - z * W;
+        float v;
+        if (z < Z)
+            v = load_param<T>(a.bq, (int64_t)c * a.H + head, a.t_f32) + load_param<T>(a.bz, (int64_t)z * a.H + head, a.t_f32);
+        else
+            v = load_param<T>(a.br, (int64_t)c * a.H + head, a.t_f32);
         tab[i] = v * kLog2e;
     }
     if (BACK)
-        for (int i = threadIdx.x; i < p.HG * classes * 32; i += blockDim.x) hist[i] = 0.f;
+        for (int i = lane; i < classes * 32; i += 32) hist[i] = 0.f;
     // columns past D stay zero: no copy writes them, and results there are zero
-    for (int i = threadIdx.x; i < 2 * p.stage / 16; i += blockDim.x)
-        reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+    for (int i = lane; i < 2 * p.stage / 16; i += 32) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
 
-    RowCopy<T, DP> in, out;
-    in.init(heads, a.D, p.row, p.vec_in);
-    out.init(heads, a.D, p.row, p.vec_out);
     const uint32_t queries = a.Nq < 32 ? (1u << a.Nq) - 1 : 0xffffffffu;
     const int64_t step = gridDim.x / p.groups;
-    const int operand = kSlots * p.row;
+    int64_t b = blockIdx.x / p.groups;
 
-    // a position's mask (in every warp) and coordinates (in warp 0), held from
-    // one turn to the next so that their loads are not waited for
+    // 16-byte copies: PIECES lanes a row, ROWS rows a pass, PIECES passes
+    constexpr int E = sizeof(T), PIECES = DP * E / 16, ROWS = 32 / PIECES;
+    const int lane_row = lane / PIECES, lane_byte = lane % PIECES * 16;
+    const bool in_row = lane_byte < a.D * E;
+    Walk wq, wk, wv, wg, oq, ok, ov;
+    if (p.vec_in) {
+        wq.init(a.q, a.qs, b, step, head, lane_row, ROWS, lane_byte, E);
+        wk.init(a.k, a.ks, b, step, head, lane_row, ROWS, lane_byte, E);
+        wv.init(a.v, a.vs, b, step, head, lane_row, ROWS, lane_byte, E);
+        if (BACK) wg.init(a.dout, a.os, b, step, head, lane_row, ROWS, lane_byte, E);
+    }
+    if (p.vec_out) {
+        oq.init(BACK ? a.dq : a.out, a.gs, b, step, head, lane_row, ROWS, lane_byte, E);
+        if (BACK) {
+            ok.init(a.dk, a.gks, b, step, head, lane_row, ROWS, lane_byte, E);
+            ov.init(a.dv, a.gks, b, step, head, lane_row, ROWS, lane_byte, E);
+        }
+    }
+
+    // a position's mask and coordinates, held from one turn to the next so that
+    // their loads are not waited for
     struct Tokens {
-        int alive;
-        int c[3];
+        int alive, c[3];
     };
     auto fetch = [&](int64_t b) {
         Tokens k = {0, {0, 0, 0}};
         if (b < a.B && lane < a.N) {
             k.alive = a.mask[b * a.ms + lane];
-            if (warp == 0) k.c[0] = a.tq[b * a.tqs + lane], k.c[1] = a.tr[b * a.trs + lane], k.c[2] = a.tz[b * a.tzs + lane];
+            k.c[0] = a.tq[b * a.tqs + lane], k.c[1] = a.tr[b * a.trs + lane], k.c[2] = a.tz[b * a.tzs + lane];
         }
         return k;
     };
     auto issue = [&](int64_t b, char* st, const Tokens& k) -> uint32_t {
         const uint32_t valid = __ballot_sync(0xffffffffu, k.alive != 0);
         if (b < a.B) {
-            if (warp == 0 && k.alive) {
+            if (k.alive) {
                 int* c = reinterpret_cast<int*>(st) + __popc(valid & ((1u << lane) - 1));
 #pragma unroll
                 for (int i = 0; i < 3; i++) c[i * kSlots] = coord(k.c[i]) * 4;
             }
             char* x = st + 3 * kSlots * 4;
-            for (int u = warp; u < (BACK ? 8 : 6); u += warps) {
-                const int o = u >> 1;
-                const void* src = o == 0 ? a.q : o == 1 ? a.k : o == 2 ? a.v : a.dout;
-                const int64_t* s = o == 0 ? a.qs : o == 1 ? a.ks : o == 2 ? a.vs : a.os;
-                in.load(x + o * operand, src, s, b, h0, o == 0 || o == 3 ? a.Nq : a.N, u & 1, valid);
+            if (p.vec_in) {
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    const int r = i * ROWS + lane_row;
+                    if (in_row && (valid >> r & 1)) {
+                        char* d = x + slot_of(valid, r) * p.row + lane_byte;
+                        if (queries >> r & 1) {
+                            cp_async16(d, wq.at + i * wq.pass);
+                            if (BACK) cp_async16(d + 3 * operand, wg.at + i * wg.pass);
+                        }
+                        cp_async16(d + operand, wk.at + i * wk.pass);
+                        cp_async16(d + 2 * operand, wv.at + i * wv.pass);
+                    }
+                }
+                wq.at += wq.turn, wk.at += wk.turn, wv.at += wv.turn;
+                if (BACK) wg.at += wg.turn;
+            } else {
+                load_rows(x, p.row, static_cast<const T*>(a.q) + b * a.qs[0] + head * a.qs[2], a.qs[1], a.Nq, a.D, valid);
+                load_rows(x + operand, p.row, static_cast<const T*>(a.k) + b * a.ks[0] + head * a.ks[2], a.ks[1], a.N, a.D, valid);
+                load_rows(x + 2 * operand, p.row, static_cast<const T*>(a.v) + b * a.vs[0] + head * a.vs[2], a.vs[1], a.N, a.D, valid);
+                if (BACK)
+                    load_rows(x + 3 * operand, p.row, static_cast<const T*>(a.dout) + b * a.os[0] + head * a.os[2], a.os[1], a.Nq,
+                              a.D, valid);
             }
+            // the slots up to the next multiple of 16 count as zero rows
+            const int n = __popc(valid), nq = __popc(valid & queries), words = p.row >> 4;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            uint4 *zq = reinterpret_cast<uint4*>(x + nq * p.row), *zk = reinterpret_cast<uint4*>(x + operand + n * p.row);
+            for (int i = lane; i < (-nq & 15) * words; i += 32) {
+                zq[i] = zero;
+                if (BACK) zq[i + 3 * (operand >> 4)] = zero;
+            }
+            for (int i = lane; i < (-n & 15) * words; i += 32) zk[i] = zk[i + (operand >> 4)] = zero;
         }
         cp_async_commit();
         return valid;
     };
 
-    int64_t b = blockIdx.x / p.groups;
     Tokens next = fetch(b);
     uint32_t valid = issue(b, stages, next);
     next = fetch(b + step);
     const float scale2 = a.scale * kLog2e;
-    const ClassOf cls = {8 * a.clip, 8 * a.clip_z};
+    Classes cls(a);
     for (int turn = 0; b < a.B; b += step, turn ^= 1) {
         char* st = stages + turn * p.stage;
         const uint32_t valid_next = issue(b + step, stages + (turn ^ 1) * p.stage, next);
         next = fetch(b + 2 * step);
         cp_async_wait<1>();
-        __syncthreads();
+        __syncwarp();
         char* x = st + 3 * kSlots * 4;
-        if (warp < heads && valid) {
-            const int n = __popc(valid), nq = __popc(valid & queries);
+        const int n = uniform(__popc(valid)), nq = uniform(__popc(valid & queries));
+        if (n) {
             const int* co = reinterpret_cast<const int*>(st);
-            T* Q = reinterpret_cast<T*>(x) + warp * DP;
-            T* K = reinterpret_cast<T*>(x + operand) + warp * DP;
-            T* V = reinterpret_cast<T*>(x + 2 * operand) + warp * DP;
-            T* G = reinterpret_cast<T*>(x + 3 * operand) + warp * DP;
-            const char* bias = reinterpret_cast<const char*>(tab + warp * classes);
-            const char* bias_r = bias + W * 4;
-            const char* bias_z = bias + 2 * W * 4;
-            const uint32_t hq = smem_addr(hist + warp * classes * 32 + lane), hr = hq + W * 128, hz = hr + W * 128;
+            T* Q = reinterpret_cast<T*>(x);
+            T* K = reinterpret_cast<T*>(x + operand);
+            T* V = reinterpret_cast<T*>(x + 2 * operand);
+            T* G = reinterpret_cast<T*>(x + 3 * operand);
+            const char* bias = reinterpret_cast<const char*>(tab);
+            const char* bias_r = bias + Z * W * 4;
+            const uint32_t hq = smem_addr(hist + lane), hr = hq + W * 128, hz = hr + W * 128;
             float dk[2][NC][4], dv[2][NC][4];
             if (BACK)
 #pragma unroll
@@ -253,35 +252,39 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                     const int2 kq = *reinterpret_cast<const int2*>(co + j), kr = *reinterpret_cast<const int2*>(co + kSlots + j),
                                kz = *reinterpret_cast<const int2*>(co + 2 * kSlots + j);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int r = e >> 1;
-                        const int cq = cls.q(e & 1 ? kq.y : kq.x, q4[r][0]), cr = cls.q(e & 1 ? kr.y : kr.x, q4[r][1]),
-                                  cz = cls.z(e & 1 ? kz.y : kz.x, q4[r][2]);
-                        const float add = *reinterpret_cast<const float*>(bias + cq) +
-                                          *reinterpret_cast<const float*>(bias_r + cr) +
-                                          *reinterpret_cast<const float*>(bias_z + cz);
-                        s[i][e] = j + (e & 1) < n ? fmaf(s[i][e], scale2, add) : -INFINITY;
-                        top[r] = fmaxf(top[r], s[i][e]);
+                    for (int r = 0; r < 2; r++) {
+                        cls.of(kq.x, kr.x, kz.x, q4[r][0], q4[r][1], q4[r][2]);
+                        const float2 ba = bias_of(bias, bias_r, cls);
+                        cls.of(kq.y, kr.y, kz.y, q4[r][0], q4[r][1], q4[r][2]);
+                        const float2 bb = bias_of(bias, bias_r, cls);
+                        const float2 x2 = fma2(make_float2(s[i][2 * r], s[i][2 * r + 1]), make_float2(scale2, scale2),
+                                               add2(make_float2(ba.x, bb.x), make_float2(ba.y, bb.y)));
+                        s[i][2 * r] = j < n ? x2.x : -INFINITY;
+                        s[i][2 * r + 1] = j + 1 < n ? x2.y : -INFINITY;
+                        top[r] = fmaxf(top[r], fmaxf(s[i][2 * r], s[i][2 * r + 1]));
                     }
                 }
-                float sum[2] = {0.f, 0.f};
+                float sum[2], delta[2] = {0.f, 0.f};
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
                     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
                 }
+                float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     if (8 * i >= n) continue;  // s stays 0 there
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        s[i][e] = exp2_approx(s[i][e] - top[e >> 1]);
-                        sum[e >> 1] += s[i][e];
+                    for (int r = 0; r < 2; r++) {
+                        float2 x2 = add2(make_float2(s[i][2 * r], s[i][2 * r + 1]), make_float2(-top[r], -top[r]));
+                        x2.x = exp2_approx(x2.x), x2.y = exp2_approx(x2.y);
+                        add[r] = add2(add[r], x2);
+                        s[i][2 * r] = x2.x, s[i][2 * r + 1] = x2.y;
                     }
                 }
-                float delta[2] = {0.f, 0.f};
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
+                    sum[r] = add[r].x + add[r].y;
                     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
                     sum[r] = rcp_approx(sum[r]);
@@ -313,17 +316,20 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                         store_vec<T, 2>(Q + (m0 + g + 8) * ld + 8 * c + 2 * t, hi);
                     }
                 } else {
+                    add[0] = add[1] = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if (8 * i >= n) continue;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            s[i][e] *= sum[e >> 1];
-                            delta[e >> 1] = fmaf(s[i][e], dp[i][e], delta[e >> 1]);
+                        for (int r = 0; r < 2; r++) {
+                            const float2 x2 = mul2(make_float2(s[i][2 * r], s[i][2 * r + 1]), make_float2(sum[r], sum[r]));
+                            add[r] = fma2(x2, make_float2(dp[i][2 * r], dp[i][2 * r + 1]), add[r]);
+                            s[i][2 * r] = x2.x, s[i][2 * r + 1] = x2.y;
                         }
                     }
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
+                        delta[r] = add[r].x + add[r].y;
                         delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 1);
                         delta[r] += __shfl_xor_sync(0xffffffffu, delta[r], 2);
                     }
@@ -331,21 +337,22 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         if (8 * i >= n) continue;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) dp[i][e] = s[i][e] * (dp[i][e] - delta[e >> 1]);
                         const int j = 8 * i + 2 * t;
                         const int2 kq = *reinterpret_cast<const int2*>(co + j), kr = *reinterpret_cast<const int2*>(co + kSlots + j),
                                    kz = *reinterpret_cast<const int2*>(co + 2 * kSlots + j);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int r = e >> 1;
-                            add_at(hq + cls.q(e & 1 ? kq.y : kq.x, q4[r][0]) * 32, hr + cls.q(e & 1 ? kr.y : kr.x, q4[r][1]) * 32,
-                                   hz + cls.z(e & 1 ? kz.y : kz.x, q4[r][2]) * 32, dp[i][e]);
+                        for (int r = 0; r < 2; r++) {
+                            float2 x2 = add2(make_float2(dp[i][2 * r], dp[i][2 * r + 1]), make_float2(-delta[r], -delta[r]));
+                            x2 = mul2(x2, make_float2(s[i][2 * r], s[i][2 * r + 1]));
+                            dp[i][2 * r] = x2.x, dp[i][2 * r + 1] = x2.y;
+                            cls.of(kq.x, kr.x, kz.x, q4[r][0], q4[r][1], q4[r][2]);
+                            add_at(hq + cls.q * 32, hr + cls.r * 32, hz + cls.z * 32, x2.x);
+                            cls.of(kq.y, kr.y, kz.y, q4[r][0], q4[r][1], q4[r][2]);
+                            add_at(hq + cls.q * 32, hr + cls.r * 32, hz + cls.z * 32, x2.y);
                         }
                     }
                     typename Op::A pt[2][16 / Op::KK][PARTS];
-                    float* room = scratch + (F32 ? warp * 16 * kTransposeLd : 0);
-                    transpose_c<T, DP == 8>(pt, s, room, lane);
+                    transpose_c<T, DP == 8>(pt, s, n, room, lane);
 #pragma unroll
                     for (int k = 0; k < 16 / Op::KK; k++)
 #pragma unroll
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                             Op::template product<false>(dv[0] + c, pt[0][k], gb);
                             if (n > 16) Op::template product<false>(dv[1] + c, pt[1][k], gb);
                         }
-                    transpose_c<T, DP == 8>(pt, dp, room, lane);
+                    transpose_c<T, DP == 8>(pt, dp, n, room, lane);
 #pragma unroll
                     for (int k = 0; k < 16 / Op::KK; k++)
 #pragma unroll
@@ -408,21 +415,41 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                     }
             }
         }
-        __syncthreads();
-        for (int u = warp; u < (BACK ? 6 : 2); u += warps) {
-            const int o = u >> 1;
-            void* dst = !BACK ? a.out : o == 0 ? a.dq : o == 1 ? a.dk : a.dv;
-            out.store(x + o * operand, dst, o == 0 ? a.gs : a.gks, b, h0, o == 0 ? a.Nq : a.N, u & 1, valid);
+        __syncwarp();
+        if (p.vec_out) {
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const int r = i * ROWS + lane_row;
+                if (in_row && r < a.N) {
+                    const char* s = x + slot_of(valid, r) * p.row + lane_byte;
+                    const bool live = valid >> r & 1;
+                    const uint4 zero = make_uint4(0, 0, 0, 0);
+                    if (queries >> r & 1)
+                        *reinterpret_cast<uint4*>(oq.at + i * oq.pass) = live ? *reinterpret_cast<const uint4*>(s) : zero;
+                    if (BACK) {
+                        *reinterpret_cast<uint4*>(ok.at + i * ok.pass) = live ? *reinterpret_cast<const uint4*>(s + operand) : zero;
+                        *reinterpret_cast<uint4*>(ov.at + i * ov.pass) = live ? *reinterpret_cast<const uint4*>(s + 2 * operand) : zero;
+                    }
+                }
+            }
+            oq.at += oq.turn;
+            if (BACK) ok.at += ok.turn, ov.at += ov.turn;
+        } else {
+            store_rows(x, p.row, static_cast<T*>(BACK ? a.dq : a.out) + b * a.gs[0] + head * a.gs[2], a.gs[1], a.Nq, a.D, valid);
+            if (BACK) {
+                store_rows(x + operand, p.row, static_cast<T*>(a.dk) + b * a.gks[0] + head * a.gks[2], a.gks[1], a.N, a.D, valid);
+                store_rows(x + 2 * operand, p.row, static_cast<T*>(a.dv) + b * a.gks[0] + head * a.gks[2], a.gks[1], a.N, a.D, valid);
+            }
         }
-        __syncthreads();
+        __syncwarp();
         valid = valid_next;
     }
     cp_async_wait<0>();
-    if (BACK && warp < heads) {
-        // this block's sums: a lane takes a class and adds up its 32 columns
-        float* part = a.partial + (int64_t)(blockIdx.x / p.groups) * classes * a.H + h0 + warp;
+    if (BACK) {
+        // this warp's sums: a lane takes a class and adds up its 32 columns
+        float* part = a.partial + (int64_t)(blockIdx.x / p.groups) * classes * a.H + head;
         for (int c = lane; c < classes; c += 32) {
-            const float* col = hist + (warp * classes + c) * 32;
+            const float* col = hist + c * 32;
             float v = 0.f;
             for (int i = 0; i < 32; i++) v += col[(i + lane) & 31];
             part[(int64_t)c * a.H] = v;

@@ -245,24 +245,27 @@ template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 1 : 2;
 
 // The transpose of 16 x 32 C tiles (rows: queries, columns: keys) as A operands
-// [2][16 / KK][part] (m = key, k = query): in registers for 16-bit types,
+// [2][16 / KK][part] (m = key, k = query); of 16 columns at a time, those that
+// begin below `columns`: in registers for 16-bit types,
 // through 16 x kTransposeLd floats of the warp's own for fp32.
 constexpr int kTransposeLd = 36;
 
 template <typename T, bool D8>
 __device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[2][16 / Tile<T, D8>::KK][kParts<T>],
-                                            const float (&c)[4][4], float* scratch, int lane) {
+                                            const float (&c)[4][4], int columns, float* scratch, int lane) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int m = 0; m < 2; m++) {
+            if (16 * m >= columns) continue;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float* v = c[2 * m + (i & 1)] + 2 * (i >> 1);
                 const uint32_t first = pack2(v[0], v[1], T());
-                const float2 f = unpack2(first, T());
+                const float2 f = unpack2(first, T()), z = add2(make_float2(v[0], v[1]), make_float2(-f.x, -f.y));
                 a[m][0][0].r[i] = transpose8(first);
-                a[m][0][1].r[i] = transpose8(pack2(v[0] - f.x, v[1] - f.y, T()));
+                a[m][0][1].r[i] = transpose8(pack2(z.x, z.y, T()));
             }
+        }
     } else {
         const int g = lane >> 2, t = lane & 3;
         __syncwarp();
@@ -276,6 +279,7 @@ __device__ __forceinline__ void transpose_c(typename Tile<T, D8>::A (&a)[2][16 /
         for (int m = 0; m < 2; m++)
 #pragma unroll
             for (int k = 0; k < 2; k++) {
+                if (16 * m >= columns) continue;
                 const float* p = scratch + (8 * k + 2 * t) * kTransposeLd + 16 * m + g;
                 auto& x = a[m][k][0];
                 split_tf32(p[0], x.hi[0], x.lo[0]);

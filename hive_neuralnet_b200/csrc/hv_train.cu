@@ -181,29 +181,31 @@ static bool attn_ok(const hv_attention* a) {
 static int attn_classes(const hv_attention* a) { return 2 * (2 * a->coord_clip + 1) + 2 * a->height_clip + 1; }
 
 // ---- up to 32 tokens
-constexpr int kShortSmem = 100 * 1024;
+constexpr int kShortSmem = 75 * 1024;
 
 static bool attn_short(const hv_attention* a) { return a->tokens <= kSlots; }
 
+static int round_up(int x, int n) { return (x + n - 1) / n * n; }
+
 static int pad_dim(int D) { return D <= 8 ? 8 : D <= 16 ? 16 : D <= 32 ? 32 : 64; }
 
-// Heads a block: up to 8 (a warp each), fewer where their rows would leave an
-// SM with less than two blocks, or where a row is more than a warp's 512 bytes.
+// Heads a block: up to 8, a warp each, fewer where that takes more than a third
+// of an SM's shared memory.
 static ShortPlan short_plan(const hv_attention* a, bool back) {
     const int e = (int)elem_bytes(a->dtype), DP = pad_dim(a->head_dim), classes = attn_classes(a);
     ShortPlan p = {};
-    for (p.groups = (a->heads + 7) / 8;; p.groups++) {
-        p.HG = (a->heads + p.groups - 1) / p.groups;
-        const int unit = e == 4 ? 32 : 16;  // rows an odd number of these apart do not meet in a bank
-        p.row = p.HG * DP * e;
-        if (p.row / unit % 2 == 0) p.row += unit;
-        p.stage = 3 * kSlots * 4 + (back ? 4 : 3) * kSlots * p.row;
-        const int floats = p.HG * classes * (back ? 33 : 1) + (back && e == 4 ? p.HG * 16 * kTransposeLd : 0);
-        p.tables = (int)((floats * 4 + 127) & ~127);
-        p.total = p.tables + 2 * p.stage;
-        if ((p.total <= kShortSmem && p.HG * a->head_dim * e <= 512) || p.HG == 1) break;
-    }
-    p.groups = (a->heads + p.HG - 1) / p.HG;
+    const int unit = e == 4 ? 32 : 16;  // rows an odd number of these apart do not meet in a bank
+    p.row = DP * e;
+    if (p.row / unit % 2 == 0) p.row += unit;
+    p.stage = 3 * kSlots * 4 + (back ? 4 : 3) * kSlots * p.row;
+    const int floats = (2 * a->height_clip + 2) * (2 * a->coord_clip + 1) + (back ? 32 * classes : 0) +
+                       (back && e == 4 ? 16 * kTransposeLd : 0);
+    p.warp = 2 * p.stage + round_up(floats * 4, 128);
+    int most = kShortSmem / p.warp;
+    most = most < 1 ? 1 : most > 8 ? 8 : most;
+    p.groups = (a->heads + most - 1) / most;
+    p.HG = (a->heads + p.groups - 1) / p.groups;
+    p.total = p.HG * p.warp;
     return p;
 }
 
@@ -255,8 +257,6 @@ static bool vec_out(const AttnArgs& x, int e, bool back) {
 
 // ---- any number of tokens
 constexpr int kKeysLeast = 32;  // keys a block, at least
-
-static int round_up(int x, int n) { return (x + n - 1) / n * n; }
 
 // What the forward pass leaves for the backward pass (or, without one, its
 // workspace: the first two alone).
