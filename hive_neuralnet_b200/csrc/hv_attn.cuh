@@ -63,6 +63,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024) k_attn_table_sum(const float* __restrict__ partial, int64_t n, int W, int classes,
                                                          int H, void* dbq, void* dbr, void* dbz, int t_f32) {
     __shared__ float sums[32][8];
+    after_previous();
     const int v = threadIdx.x & 7, part = threadIdx.x >> 3, at = blockIdx.x * 8 + v, values = classes * H;
     float x = 0.f;
     if (at < values)

@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
     const int64_t b = blockIdx.x / l.tiles / a.H;
+    load_bias_table<T>(smem, a, h);  // the caller's: nothing that the kernel before writes
+    after_previous();
     const int2 count = l.count[b];
     const int q0 = tile * ROWS, n = count.x, nq = count.y - q0;  // nq: this tile's valid queries, if below ROWS
     const int4* meta = l.meta + b * l.Npad;
@@ -170,7 +172,6 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
         cp_async_commit();
     };
     issue(0);
-    load_bias_table<T>(smem, a, h);
 
     const int part = warp % WK, row0 = warp / WK * 16, key0 = part * (kTile / WK);
     const float scale2 = a.scale * kLog2E;
@@ -419,6 +420,9 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
     const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
     const int64_t b = blockIdx.x / l.tiles / a.H;
     const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
+    load_bias_table<T>(smem, a, h);
+    for (int i = threadIdx.x; i < classes * THREADS; i += THREADS) hist[i] = 0.f;
+    after_previous();
     const int2 count = l.count[b];
     const int k0 = tile * KEYS, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below KEYS
     const int4* meta = l.meta + b * l.Npad;
@@ -464,8 +468,6 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
         cp_async_commit();
     };
     issue(0);
-    load_bias_table<T>(smem, a, h);
-    for (int i = threadIdx.x; i < classes * THREADS; i += THREADS) hist[i] = 0.f;
     const float scale2 = a.scale * kLog2E;
     const uint32_t hq = smem_addr(hist + warp * classes * 32 + lane), hr = hq + W * 128, hz = hr + W * 128;
     Classes cls(a);

@@ -82,19 +82,23 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
     float* room = reinterpret_cast<float*>(stages + 2 * p.stage);
     float* tab = room + (BACK && F32 ? 16 * kTransposeLd : 0);
     float* hist = tab + (Z + 1) * W;
+#pragma unroll 4
     for (int i = lane; i < (Z + 1) * W; i += 32) {
         const int z = i / W, c = i - z * W;
-        float v;
-        if (z < Z)
-            v = load_param<T>(a.bq, (int64_t)c * a.H + head, a.t_f32) + load_param<T>(a.bz, (int64_t)z * a.H + head, a.t_f32);
-        else
-            v = load_param<T>(a.br, (int64_t)c * a.H + head, a.t_f32);
+        float v = load_param<T>(z < Z ? a.bq : a.br, (int64_t)c * a.H + head, a.t_f32);
+        if (z < Z) v += load_param<T>(a.bz, (int64_t)z * a.H + head, a.t_f32);
         tab[i] = v * kLog2e;
     }
     if (BACK)
+#pragma unroll 8
         for (int i = lane; i < classes * 32; i += 32) hist[i] = 0.f;
-    // columns past D stay zero: no copy writes them, and results there are zero
-    for (int i = lane; i < 2 * p.stage / 16; i += 32) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
+    // The coordinates of slots past the last token are read (for pairs that are
+    // then dropped) and index the tables, so they must be multiples of 4 from the
+    // start.  Columns past D stay zero: no copy writes them, results there are zero.
+    for (int i = lane; i < 3 * kSlots; i += 32)
+        reinterpret_cast<int*>(stages)[i] = reinterpret_cast<int*>(stages + p.stage)[i] = 0;
+    if (a.D < DP)
+        for (int i = lane; i < 2 * p.stage / 16; i += 32) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
     __syncwarp();
 
     const uint32_t queries = a.Nq < 32 ? (1u << a.Nq) - 1 : 0xffffffffu;

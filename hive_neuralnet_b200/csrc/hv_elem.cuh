@@ -22,6 +22,10 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// In a kernel launched to overlap the end of the one before it on its stream:
+// waits for that one to have finished.  Returns at once in any other.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // N consecutive elements moved as one memory word (N * sizeof(T) bytes, a
 // power of two up to 16, naturally aligned).
 template <typename T, int N>

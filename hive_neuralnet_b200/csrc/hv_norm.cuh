@@ -364,6 +364,7 @@ template <typename T>
 __global__ void __launch_bounds__(1024) k_norm_reduce(const float* __restrict__ partial, int n, int C, void* dw,
                                                       void* db, int w_f32) {
     __shared__ float sums[32][8];
+    after_previous();
     const int v = threadIdx.x & 7, part = threadIdx.x >> 3, col = blockIdx.x * 8 + v;
     float x = 0.f;
     if (col < 2 * C)

@@ -59,6 +59,19 @@ static int resident_blocks(K kernel, int threads, int smem, int* out) {
     return HV_OK;
 }
 
+// A launch that may begin while the kernel before it on the stream ends; the
+// kernel calls after_previous() before it reads what that one wrote.
+template <typename... P, typename... A>
+static int launch_after(void (*kernel)(P...), unsigned grid, int threads, int smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute overlap = {};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid), c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = st;
+    c.attrs = &overlap, c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess ? HV_OK : (cudaGetLastError(), HV_ECUDA);
+}
+
 // Calls f with a value of the element type.
 template <typename F>
 static int by_type(int dtype, F f) {
@@ -232,9 +245,8 @@ static int launch_short(const AttnArgs& x, ShortPlan p, cudaStream_t st) {
         const int rc2 = launched();
         if (rc2 || !BACK) return rc2;
         const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
-        k_attn_table_sum<T><<<(classes * x.H + 7) / 8, 1024, 0, st>>>(x.partial, p.per_group, W, classes, x.H, x.dbq, x.dbr,
-                                                                     x.dbz, x.t_f32);
-        return launched();
+        return launch_after(k_attn_table_sum<T>, (classes * x.H + 7) / 8, 1024, 0, st, x.partial, p.per_group, W, classes, x.H,
+                            x.dbq, x.dbr, x.dbz, x.t_f32);
     };
     switch (pad_dim(x.D)) {
         case 8: return go(k_attn_short<T, 8, BACK>);
@@ -298,6 +310,8 @@ static int launch_query(const AttnArgs& x, LongArgs l, cudaStream_t st) {
     int n = 0;
     const int rc = resident_blocks(k_attn_query<T, DP, ROWS, WK, BACK>, threads, smem, &n);
     if (rc) return rc;
+    if (!BACK)  // after the sort; the tables, which it reads before that has ended, are older
+        return launch_after(k_attn_query<T, DP, ROWS, WK, BACK>, (unsigned)grid, threads, smem, st, x, l);
     k_attn_query<T, DP, ROWS, WK, BACK><<<(unsigned)grid, threads, smem, st>>>(x, l);
     return launched();
 }
@@ -315,12 +329,10 @@ static int launch_keys(const AttnArgs& x, LongArgs l, cudaStream_t st) {
     int rc = resident_blocks(k_attn_keys<T, DP, KEYS, WQ>, threads, smem, &n);
     if (rc) return rc;
     if (grid) {
-        k_attn_keys<T, DP, KEYS, WQ><<<(unsigned)grid, threads, smem, st>>>(x, l);
-        if ((rc = launched())) return rc;
+        if ((rc = launch_after(k_attn_keys<T, DP, KEYS, WQ>, (unsigned)grid, threads, smem, st, x, l))) return rc;
     }
-    k_attn_table_sum<T><<<(classes * x.H + 7) / 8, 1024, 0, st>>>(x.partial, x.B * l.tiles, W, classes, x.H, x.dbq, x.dbr, x.dbz,
-                                                                 x.t_f32);
-    return launched();
+    return launch_after(k_attn_table_sum<T>, (classes * x.H + 7) / 8, 1024, 0, st, x.partial, x.B * l.tiles, W, classes, x.H, x.dbq,
+                        x.dbr, x.dbz, x.t_f32);
 }
 
 // 64 queries (keys) a block.  With too few such blocks to give every scheduler
@@ -421,8 +433,7 @@ int hv_layer_norm_backward(const void* dy, const void* x, const void* weight, co
             const int rc = dsum ? launch_norm<T, true, true>(a, s, &grid, st) : launch_norm<T, true, false>(a, s, &grid, st);
             if (rc || grid == 1) return rc;
         }
-        k_norm_reduce<T><<<(2 * width + 7) / 8, 1024, 0, st>>>(a.partial, grid, width, dweight, dbias, a.w_f32);
-        return launched();
+        return launch_after(k_norm_reduce<T>, (2 * width + 7) / 8, 1024, 0, st, a.partial, grid, width, dweight, dbias, a.w_f32);
     });
 }
 
