@@ -4,7 +4,9 @@
 
 #include <cstdint>
 #include <initializer_list>
+#include <map>
 #include <mutex>
+#include <tuple>
 #include <type_traits>
 
 #include "hv_adamw.cuh"
@@ -37,26 +39,30 @@ static int sm_count() {
 
 constexpr int kSmemPerSm = 228 * 1024, kSmemPerBlock = 227 * 1024;
 
-// Shared-memory limit and resident blocks of a kernel, asked for once per
-// device and shape.
+// Resident blocks of a kernel on an SM, asked for once for each device, kernel
+// and shape; the kernel's shared-memory limit is raised on the way.
 template <typename K>
 static int resident_blocks(K kernel, int threads, int smem, int* out) {
-    struct Known { int threads, smem, blocks; };
-    static Known known[64];
+    static std::map<std::tuple<int, const void*, int, int>, int> known;
     static std::mutex mu;
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HV_ECUDA;
-    std::lock_guard<std::mutex> lock(mu);
-    Known& k = known[dev];
-    if (!k.blocks || k.threads != threads || k.smem != smem) {
-        if (smem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock) != cudaSuccess)
-            return HV_ECUDA;
-        int n = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) return HV_ECUDA;
-        k = {threads, smem, n};
+    if (cudaGetDevice(&dev) != cudaSuccess) return cudaGetLastError(), HV_ECUDA;
+    try {
+        std::lock_guard<std::mutex> lock(mu);
+        int& n = known[{dev, reinterpret_cast<const void*>(kernel), threads, smem}];
+        if (!n) {
+            if (smem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerBlock) != cudaSuccess)
+                return cudaGetLastError(), HV_ECUDA;
+            int blocks = 0;
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, smem) != cudaSuccess || blocks < 1)
+                return cudaGetLastError(), HV_ECUDA;
+            n = blocks;
+        }
+        *out = n;
+        return HV_OK;
+    } catch (...) {  // no memory for the entry
+        return HV_ECUDA;
     }
-    *out = k.blocks;
-    return HV_OK;
 }
 
 // A launch that may begin while the kernel before it on the stream ends; the

@@ -202,6 +202,64 @@ def test_attention_empty():
         assert not any(g.any() for g in grads)
 
 
+def test_attention_no_queries_of_many_tokens():
+    qkv, where, tables, dout = attention_inputs(2, 40, 0, 3, 8, torch.float32)
+    got = check_attention(qkv[:, :0, 0], qkv[:, :, 1], qkv[:, :, 2], where, tables, dout)
+    assert not any(t.any() for t in got[2:])
+
+
+@pytest.mark.parametrize("n", [29, 70])
+def test_attention_tables_written_just_before(n):
+    """Each pass follows at once on the kernels that write its bias tables and operands."""
+    from hive_neuralnet_b200 import train_ops as ops
+    qkv, where, tables, dout = attention_inputs(40, n, n, 8, 16, torch.bfloat16)
+    out, saved = ops.relative_attention_forward(*qkv.unbind(2), *where, *tables, save=True)
+    want = [out, *ops.relative_attention_backward(dout, *qkv.unbind(2), *where, *tables, saved)]
+    late, spare = [t.clone() for t in tables], torch.zeros(50_000_000, device="cuda")
+    for _ in range(3):
+        for t in late:
+            t.zero_()
+        torch.cuda.synchronize()
+        spare.add_(1)
+        for t, value in zip(late, tables):
+            t.copy_(value)
+        out, saved = ops.relative_attention_forward(*qkv.unbind(2), *where, *late, save=True)
+        for t in late:
+            t.zero_()
+        spare.add_(1)
+        for t, value in zip(late, tables):
+            t.copy_(value)
+        got = [out, *ops.relative_attention_backward(dout, *qkv.unbind(2), *where, *late, saved)]
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_types_in_turn_in_a_new_process():
+    """A kernel's first launch in a process, of one type after another at the same shape."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from hive_neuralnet_b200 import train_ops as ops
+for n in (29, 70):
+    for dtype in (torch.float16, torch.bfloat16, torch.float32, torch.float16):
+        qkv = torch.ones(3, n, 3, 8, 64, device='cuda', dtype=dtype)
+        at, mask = torch.zeros(3, n, dtype=torch.int32, device='cuda'), torch.ones(3, n, dtype=torch.bool, device='cuda')
+        tables = [torch.zeros(17, 8, device='cuda'), torch.zeros(17, 8, device='cuda'), torch.zeros(5, 8, device='cuda')]
+        q, k, v = qkv.unbind(2)
+        out, saved = ops.relative_attention_forward(q, k, v, at, at, at, mask, *tables, save=True)
+        grads = ops.relative_attention_backward(out, q, k, v, at, at, at, mask, *tables, saved)
+        assert (out.float() - 1).abs().max().item() < 1e-2 and grads[0].abs().max().item() < 1e-2
+        x = qkv.reshape(-1, 64)
+        y, s, mean, rstd = ops.layer_norm_forward(x, torch.ones(64, device='cuda'), torch.zeros(64, device='cuda'))
+        ops.layer_norm_backward(y, s, torch.ones(64, device='cuda'), mean, rstd)
+        torch.cuda.synchronize()
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_attention_offsets_past_32_bits():
     """Batch strides over 2^31 elements."""
     b, n, h, d = 2, 29, 8, 8
