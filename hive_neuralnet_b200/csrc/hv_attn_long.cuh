@@ -5,14 +5,24 @@
 // with their coordinates; everything after works on those slots, so a masked
 // token costs nothing but the zeros of its results.
 //
-// Forward and dq: a block takes 64 queries of one head, 16 a warp, and walks
-// over tiles of 64 keys, the next tile arriving while this one is computed.
-// With few queries a block takes 16 and its warps share each tile's keys; their
-// parts are joined at the end.  dk, dv: a block takes 64 keys, 16 a warp, and
-// walks over the queries with the scores transposed (rows: keys), so that the
-// probabilities are operands of both products as they stand.  The scores are
-// computed once more there: the sums over queries and over keys are both taken
-// in registers, in a fixed order, with no atomics.
+// Forward and dq: a block of four warps takes 32 queries of one head and walks
+// over tiles of 64 keys, the next tile arriving while this one is computed; a
+// warp takes 16 queries and half of each tile's keys.  With few queries a block
+// takes 16, a warp a quarter of the keys.  The warps' parts are joined at the
+// end, in their order.  dk, dv: a block takes 32 keys, a warp 16 of them and
+// half of each tile of queries, with the scores transposed (rows: keys), so
+// that the probabilities are operands of both products as they stand.  The
+// scores are computed once more there: the sums over queries and over keys are
+// both taken in registers, in a fixed order, with no atomics.
+//
+// A score costs about 25 (forward), 25 (dq) and 50 (keys) warp instructions
+// for each 32 of them beside its products: classes, two table lookups, the
+// exponential, the split into two parts, the bias sums.  With 64 values a head
+// the products take a third of the tensor pipe's time in that; the kernels wait
+// on their own dependences (two to four warps a scheduler), not on memory.
+// 2 x 1023 tokens, 8 heads of 64, bf16, 768 valid tokens on average: forward
+// 50 us, backward 112 us.  Blocks of 64 rows with whole rows a warp were up to
+// 40 % slower below two waves of blocks and 5 % faster above four.
 #pragma once
 
 #include "hv_attn.cuh"
@@ -20,7 +30,7 @@
 
 namespace hv {
 
-constexpr int kTile = 64;          // tokens of a tile
+constexpr int kTile = 64;  // tokens of a tile
 constexpr float kLog2E = 1.4426950408889634f;
 
 struct LongArgs {
@@ -117,9 +127,10 @@ __device__ __forceinline__ void load_bias_table(char* smem, const AttnArgs& a, i
 // BACK false: the forward pass; true: dq (and delta).  A warp takes 16 of the
 // ROWS queries and 1 / WK of each tile's keys.
 template <typename T, int DP, int ROWS, int WK, bool BACK>
-__global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, const LongArgs l) {
+__global__ void __launch_bounds__(128, ROWS == 32 ? 5 : 1) k_attn_query(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
-    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = ROWS * 2 * WK;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = 128;
+    static_assert(ROWS * 2 * WK == THREADS, "a warp for each 16 queries and part of the keys");
     constexpr int NT = 8 / WK;          // 8-key tiles of a warp
     constexpr int NB = NT < 4 ? NT : 4, CB = sizeof(T) == 4 && NC > 4 ? 4 : NC;
     // The output before rounding gives the backward pass its sum_j p dp, which it
@@ -398,25 +409,26 @@ __global__ void __launch_bounds__(ROWS * 2 * WK) k_attn_query(const AttnArgs a, 
     }
 }
 
-// dk, dv and the bias sums of KEYS keys of one head.  A warp takes 16 of the
-// keys and, of each tile's queries, 32 at a time: all of them in turn, or (WQ =
-// 2) one half.
-template <typename T, int DP, int KEYS, int WQ>
-__global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, const LongArgs l) {
+// dk, dv and the bias sums of 32 keys of one head.  A warp takes 16 of the keys
+// and one half of each tile's queries.
+constexpr int kKeys = 32, kKeyThreads = 128;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kKeyThreads, 3) k_attn_keys(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
-    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, CB = NC < 4 ? NC : 4, THREADS = 2 * KEYS * WQ, PARTS = kParts<T>;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, CB = NC < 4 ? NC : 4, THREADS = kKeyThreads, PARTS = kParts<T>;
     extern __shared__ __align__(16) char smem[];
     T* sk = reinterpret_cast<T*>(smem + kTabBytes);
-    T* sv = sk + KEYS * LD;
-    T* sq = sv + KEYS * LD;  // two stages of q, then of dout
+    T* sv = sk + kKeys * LD;
+    T* sq = sv + kKeys * LD;  // two stages of q, then of dout
     T* sg = sq + 2 * kTile * LD;
     int4* sm = reinterpret_cast<int4*>(sg + 2 * kTile * LD);  // three tiles of query meta
     int4* km = sm + 3 * kTile;                                // the keys' meta
-    float2* sd = reinterpret_cast<float2*>(km + KEYS);       // two tiles of (lse, -delta)
+    float2* sd = reinterpret_cast<float2*>(km + kKeys);       // two tiles of (lse, -delta)
     float* hist = reinterpret_cast<float*>(sd + 2 * kTile);   // [warp][class][lane]
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int key0 = warp % (KEYS / 16) * 16, half = warp / (KEYS / 16);
+    const int key0 = warp % 2 * 16, half = warp / 2;
     const int tile = blockIdx.x % l.tiles, h = blockIdx.x / l.tiles % a.H;
     const int64_t b = blockIdx.x / l.tiles / a.H;
     const int W = 2 * a.clip + 1, classes = 2 * W + 2 * a.clip_z + 1;
@@ -424,14 +436,14 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
     for (int i = threadIdx.x; i < classes * THREADS; i += THREADS) hist[i] = 0.f;
     after_previous();
     const int2 count = l.count[b];
-    const int k0 = tile * KEYS, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below KEYS
+    const int k0 = tile * kKeys, n = count.x - k0, nq = count.y;  // n: this tile's valid keys, if below kKeys
     const int4* meta = l.meta + b * l.Npad;
     const int64_t head = b * a.H + h;
     float* part = a.partial + ((b * l.tiles + tile) * classes) * a.H + h;
     T* dk = static_cast<T*>(a.dk) + b * a.gks[0] + h * a.gks[2];
     T* dv = static_cast<T*>(a.dv) + b * a.gks[0] + h * a.gks[2];
-    if (n < KEYS)  // masked keys: zeros
-        for (int i = threadIdx.x; i < KEYS * a.D; i += THREADS) {
+    if (n < kKeys)  // masked keys: zeros
+        for (int i = threadIdx.x; i < kKeys * a.D; i += THREADS) {
             const int r = i / a.D, d = i - r * a.D;
             if (r >= n && k0 + r < a.N) {
                 const int64_t at = meta[k0 + r].w * a.gks[1] + d;
@@ -444,11 +456,11 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
     }
     const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[2];
     const T* go = static_cast<const T*>(a.dout) + b * a.os[0] + h * a.os[2];
-    for (int i = threadIdx.x; i < KEYS; i += THREADS) km[i] = meta[k0 + i];
+    for (int i = threadIdx.x; i < kKeys; i += THREADS) km[i] = meta[k0 + i];
     for (int i = threadIdx.x; i < kTile; i += THREADS) sm[i] = meta[i];
     __syncthreads();
-    load_tile<T, DP, KEYS, THREADS>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
-    load_tile<T, DP, KEYS, THREADS>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, kKeys, THREADS>(sk, static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[2], a.ks[1], a.D, km, n, l.vec_in);
+    load_tile<T, DP, kKeys, THREADS>(sv, static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[2], a.vs[1], a.D, km, n, l.vec_in);
     const int tiles = (nq + kTile - 1) / kTile;
     auto issue = [&](int i) {
         if (i < tiles) {
@@ -489,9 +501,8 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
         cp_async_wait<0>();
         __syncthreads();
         issue(i + 1);
-#pragma unroll 1
-        for (int y = 32 * half; y < kTile; y += 32 * WQ) {
-            if (i * kTile + y >= nq || key0 >= n) break;
+        const int y = 32 * half;
+        if (i * kTile + y < nq && key0 < n) {
             const T* tq = sq + ((i & 1) * kTile + y) * LD;
             const T* tg = sg + ((i & 1) * kTile + y) * LD;
             const int4* tm = sm + i % 3 * kTile + y;
@@ -557,7 +568,7 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
     }
     cp_async_wait<0>();
     __syncthreads();
-    if (WQ > 1) {  // the halves' sums, first half first
+    {  // the halves' sums, first half first
         float* join = reinterpret_cast<float*>(smem + kTabBytes) + (key0 + g) * 2 * DP + 2 * t;
         if (half)
 #pragma unroll
@@ -607,7 +618,7 @@ __global__ void __launch_bounds__(2 * KEYS * WQ) k_attn_keys(const AttnArgs a, c
     __syncthreads();
     for (int c = threadIdx.x; c < classes; c += THREADS) {
         float x = 0.f;
-        for (int w = 0; w < KEYS / 16 * WQ; w++) x += hist[(w * classes + c) * 32];
+        for (int w = 0; w < THREADS / 32; w++) x += hist[(w * classes + c) * 32];
         part[(int64_t)c * a.H] = x;
     }
 }

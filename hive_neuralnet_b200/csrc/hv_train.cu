@@ -274,8 +274,6 @@ static bool vec_out(const AttnArgs& x, int e, bool back) {
 }
 
 // ---- any number of tokens
-constexpr int kKeysLeast = 32;  // keys a block, at least
-
 // What the forward pass leaves for the backward pass (or, without one, its
 // workspace: the first two alone).
 static size_t long_saved(const hv_attention* a, void* base, bool all, LongArgs* l) {
@@ -300,7 +298,7 @@ static size_t long_saved(const hv_attention* a, void* base, bool all, LongArgs* 
 
 static size_t long_workspace(const hv_attention* a, void* base, LongArgs* l, float** partial) {
     const size_t delta = round256((size_t)a->batch * a->heads * round_up(a->queries, kTile) * 4);
-    const int64_t blocks = a->batch * (round_up(a->tokens, kTile) / kKeysLeast);
+    const int64_t blocks = a->batch * (round_up(a->tokens, kTile) / kKeys);
     l->delta = static_cast<float*>(base);
     *partial = base ? reinterpret_cast<float*>(static_cast<char*>(base) + delta) : nullptr;
     return delta + (size_t)blocks * attn_classes(a) * a->heads * 4;
@@ -308,7 +306,7 @@ static size_t long_workspace(const hv_attention* a, void* base, LongArgs* l, flo
 
 template <typename T, int DP, int ROWS, int WK, bool BACK>
 static int launch_query(const AttnArgs& x, LongArgs l, cudaStream_t st) {
-    constexpr int LD = tile_ld<T, DP>(), threads = ROWS * 2 * WK;
+    constexpr int LD = tile_ld<T, DP>(), threads = 128;
     const int smem = kTabBytes + (ROWS * (BACK ? 2 : 1) + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + ROWS) * 16;
     l.tiles = (x.Nq + ROWS - 1) / ROWS;
     const int64_t grid = x.B * x.H * l.tiles;
@@ -322,42 +320,38 @@ static int launch_query(const AttnArgs& x, LongArgs l, cudaStream_t st) {
     return launched();
 }
 
-template <typename T, int DP, int KEYS, int WQ>
+template <typename T, int DP>
 static int launch_keys(const AttnArgs& x, LongArgs l, cudaStream_t st) {
-    constexpr int LD = tile_ld<T, DP>(), threads = 2 * KEYS * WQ;
+    constexpr int LD = tile_ld<T, DP>(), threads = kKeyThreads;
     const int W = 2 * x.clip + 1, classes = 2 * W + 2 * x.clip_z + 1;
     const int smem =
-        kTabBytes + (2 * KEYS + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + KEYS) * 16 + 2 * kTile * 8 + classes * 4 * threads;
-    l.tiles = (x.N + KEYS - 1) / KEYS;
+        kTabBytes + (2 * kKeys + 4 * kTile) * LD * (int)sizeof(T) + (3 * kTile + kKeys) * 16 + 2 * kTile * 8 + classes * 4 * threads;
+    l.tiles = (x.N + kKeys - 1) / kKeys;
     const int64_t grid = x.B * x.H * l.tiles;
     if (grid > 0x7fffffff) return HV_EINVAL;
     int n = 0;
-    int rc = resident_blocks(k_attn_keys<T, DP, KEYS, WQ>, threads, smem, &n);
+    int rc = resident_blocks(k_attn_keys<T, DP>, threads, smem, &n);
     if (rc) return rc;
     if (grid) {
-        if ((rc = launch_after(k_attn_keys<T, DP, KEYS, WQ>, (unsigned)grid, threads, smem, st, x, l))) return rc;
+        if ((rc = launch_after(k_attn_keys<T, DP>, (unsigned)grid, threads, smem, st, x, l))) return rc;
     }
     return launch_after(k_attn_table_sum<T>, (classes * x.H + 7) / 8, 1024, 0, st, x.partial, x.B * l.tiles, W, classes, x.H, x.dbq,
                         x.dbr, x.dbz, x.t_f32);
 }
 
-// 64 queries (keys) a block.  With too few such blocks to give every scheduler
-// several warps, two warps share each 16 of them; with too few for the SMs, or
-// few queries, a block takes 16 queries and four warps share them.
+// 16 queries a block where there are no more, or where blocks of 32 would leave
+// SMs without one (1 x 1024 tokens, 1 head: 26 against 31 us forward).
 template <typename T, bool BACK>
 static int launch_long(const AttnArgs& x, const LongArgs& l, cudaStream_t st) {
-    const int64_t heads = x.B * x.H, q_blocks = heads * ((x.Nq + kTile - 1) / kTile), k_blocks = heads * ((x.N + kTile - 1) / kTile);
-    const int sms = sm_count();
+    const int64_t q_blocks = x.B * x.H * ((x.Nq + 31) / 32);
     auto go = [&](auto dim) -> int {
         constexpr int DP = decltype(dim)::value;
         int rc = HV_OK;
-        if (q_blocks) {
-            if (x.Nq <= 16 || q_blocks < sms / 2) rc = launch_query<T, DP, 16, 4, BACK>(x, l, st);
-            else if (q_blocks < 4 * sms) rc = launch_query<T, DP, 32, 2, BACK>(x, l, st);
-            else rc = launch_query<T, DP, 64, 1, BACK>(x, l, st);
-        }
+        if (q_blocks)
+            rc = x.Nq <= 16 || q_blocks < sm_count() ? launch_query<T, DP, 16, 4, BACK>(x, l, st)
+                                                    : launch_query<T, DP, 32, 2, BACK>(x, l, st);
         if constexpr (BACK)
-            if (!rc) rc = k_blocks < 4 * sms ? launch_keys<T, DP, 32, 2>(x, l, st) : launch_keys<T, DP, 64, 1>(x, l, st);
+            if (!rc) rc = launch_keys<T, DP>(x, l, st);
         return rc;
     };
     switch (pad_dim(x.D)) {
