@@ -21,8 +21,9 @@
 // the products take a third of the tensor pipe's time in that; the kernels wait
 // on their own dependences (two to four warps a scheduler), not on memory.
 // 2 x 1023 tokens, 8 heads of 64, bf16, 768 valid tokens on average: forward
-// 50 us, backward 112 us.  Blocks of 64 rows with whole rows a warp were up to
-// 40 % slower below two waves of blocks and 5 % faster above four.
+// 52 us, backward 112 us.  Blocks of 64 queries (keys) with whole rows a warp:
+// 118 + 238 against 71 + 214 us at 1,000 x 40 tokens (8 heads of 8), 114 + 296
+// against 120 + 310 us at 1,024 tokens with 64 heads of 64.
 #pragma once
 
 #include "hv_attn.cuh"
@@ -124,15 +125,48 @@ __device__ __forceinline__ void load_bias_table(char* smem, const AttnArgs& a, i
     }
 }
 
+// acc += c times the KS rows of DP values at p; c: 16 x KS score tiles.  The
+// tensor core cuts its sums off instead of rounding them: for fp32 each call
+// starts from zero and is added to the running sums with rounding, or hundreds
+// of tiles would leave an error of 2e-6.
+template <typename T, int DP, int KS, int PARTS>
+__device__ __forceinline__ void add_product(float (&acc)[DP / 8][4], const float (*c)[4], const T* p, int lane) {
+    using Op = Tile<T, DP == 8>;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, CB = NC < 4 ? NC : 4;
+    constexpr bool F32 = sizeof(T) == 4;
+    float part[F32 ? NC : 1][4];
+#pragma unroll
+    for (int x = 0; x < KS; x += Op::KK) {
+        typename Op::A a[PARTS];
+        Op::a_from_c(a, c + x / 8);
+#pragma unroll
+        for (int d = 0; d < NC; d += CB) {
+            typename Op::B b[CB];
+            Op::load_bk(b, p + x * LD + 8 * d, LD, lane);
+            if constexpr (!F32) Op::template product<false>(acc + d, a, b);
+            else if (x == 0) Op::template product<true>(part + d, a, b);
+            else Op::template product<false>(part + d, a, b);
+        }
+    }
+    if constexpr (F32)
+#pragma unroll
+        for (int d = 0; d < NC; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float2 z = add2(make_float2(acc[d][e], acc[d][e + 1]), make_float2(part[d][e], part[d][e + 1]));
+                acc[d][e] = z.x, acc[d][e + 1] = z.y;
+            }
+}
+
 // BACK false: the forward pass; true: dq (and delta).  A warp takes 16 of the
 // ROWS queries and 1 / WK of each tile's keys.
 template <typename T, int DP, int ROWS, int WK, bool BACK>
-__global__ void __launch_bounds__(128, ROWS == 32 ? 5 : 1) k_attn_query(const AttnArgs a, const LongArgs l) {
+__global__ void __launch_bounds__(128, ROWS == 16 ? 1 : sizeof(T) == 4 ? 3 : 5) k_attn_query(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
     constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = 128;
     static_assert(ROWS * 2 * WK == THREADS, "a warp for each 16 queries and part of the keys");
     constexpr int NT = 8 / WK;          // 8-key tiles of a warp
-    constexpr int NB = NT < 4 ? NT : 4, CB = sizeof(T) == 4 && NC > 4 ? 4 : NC;
+    constexpr int NB = NT < 4 ? NT : 4;
     // The output before rounding gives the backward pass its sum_j p dp, which it
     // takes from every dp: there the probabilities need all 24 bits.
     constexpr int PARTS = BACK || sizeof(T) == 4 ? kParts<T> : __is_same(T, __half) ? 2 : 3;
@@ -320,18 +354,7 @@ __global__ void __launch_bounds__(128, ROWS == 32 ? 5 : 1) k_attn_query(const At
                     s[j][2 * r] = x.x, s[j][2 * r + 1] = x.y;
                 }
         }
-        const T* tb = BACK ? tk : tv;
-#pragma unroll
-        for (int x = 0; x < NT * 8; x += Op::KK) {
-            typename Op::A pa[PARTS];
-            Op::a_from_c(pa, s + x / 8);
-#pragma unroll
-            for (int c = 0; c < NC; c += CB) {
-                typename Op::B vb[CB];
-                Op::load_bk(vb, tb + x * LD + 8 * c, LD, lane);
-                Op::template product<false>(acc + c, pa, vb);
-            }
-        }
+        add_product<T, DP, NT * 8, PARTS>(acc, s, BACK ? tk : tv, lane);
     }
     cp_async_wait<0>();
 #pragma unroll
@@ -414,9 +437,9 @@ __global__ void __launch_bounds__(128, ROWS == 32 ? 5 : 1) k_attn_query(const At
 constexpr int kKeys = 32, kKeyThreads = 128;
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kKeyThreads, 3) k_attn_keys(const AttnArgs a, const LongArgs l) {
+__global__ void __launch_bounds__(kKeyThreads, sizeof(T) == 4 && DP == 64 ? 2 : 3) k_attn_keys(const AttnArgs a, const LongArgs l) {
     using Op = Tile<T, DP == 8>;
-    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, CB = NC < 4 ? NC : 4, THREADS = kKeyThreads, PARTS = kParts<T>;
+    constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = kKeyThreads, PARTS = kParts<T>;
     extern __shared__ __align__(16) char smem[];
     T* sk = reinterpret_cast<T*>(smem + kTabBytes);
     T* sv = sk + kKeys * LD;
@@ -546,24 +569,8 @@ __global__ void __launch_bounds__(kKeyThreads, 3) k_attn_keys(const AttnArgs a, 
                     add_at(hq + cb.q * 32, hr + cb.r * 32, hz + cb.z * 32, ds.y);
                 }
             }
-#pragma unroll
-            for (int x = 0; x < 32; x += Op::KK) {
-                typename Op::A pa[PARTS];
-                Op::a_from_c(pa, s + x / 8);
-#pragma unroll
-                for (int c = 0; c < NC; c += CB) {
-                    typename Op::B gb[CB];
-                    Op::load_bk(gb, tg + x * LD + 8 * c, LD, lane);
-                    Op::template product<false>(av + c, pa, gb);
-                }
-                Op::a_from_c(pa, dp + x / 8);
-#pragma unroll
-                for (int c = 0; c < NC; c += CB) {
-                    typename Op::B qb[CB];
-                    Op::load_bk(qb, tq + x * LD + 8 * c, LD, lane);
-                    Op::template product<false>(ak + c, pa, qb);
-                }
-            }
+            add_product<T, DP, 32, PARTS>(av, s, tg, lane);
+            add_product<T, DP, 32, PARTS>(ak, dp, tq, lane);
         }
     }
     cp_async_wait<0>();

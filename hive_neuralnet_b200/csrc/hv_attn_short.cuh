@@ -16,6 +16,13 @@
 // Bias-table gradients: every lane adds into its own column of a [class][lane]
 // table in shared memory for all positions its warp takes; the columns are
 // summed once at the end, in a fixed order.
+//
+// Bound by instruction issue: 890 warp instructions a position and head
+// forward, 1,524 backward at 15.5 valid tokens (issue active 74 % and 62 %,
+// tensor pipe under 10 %).  8,192 positions of 29 slots, 8 heads of 8, fp16:
+// 84 us forward, 169 us backward, where the bytes take 10 and 19 us.  Taking
+// half the heads a block, or registers for five or six blocks of four warps
+// (they spill), was no faster or slower.
 #pragma once
 
 #include "hv_attn.cuh"
