@@ -126,15 +126,15 @@ __device__ __forceinline__ void load_bias_table(char* smem, const AttnArgs& a, i
 }
 
 // acc += c times the KS rows of DP values at p; c: 16 x KS score tiles.  The
-// tensor core cuts its sums off instead of rounding them: for fp32 each call
-// starts from zero and is added to the running sums with rounding, or hundreds
-// of tiles would leave an error of 2e-6.
-template <typename T, int DP, int KS, int PARTS>
+// tensor core cuts its sums off instead of rounding them: FRESH calls start from
+// zero and are added to the running sums with rounding, where hundreds of tiles
+// would leave an error of 2e-6 (fp32, and the output that the bias gradients
+// depend on).
+template <typename T, int DP, int KS, int PARTS, bool FRESH>
 __device__ __forceinline__ void add_product(float (&acc)[DP / 8][4], const float (*c)[4], const T* p, int lane) {
     using Op = Tile<T, DP == 8>;
     constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, CB = NC < 4 ? NC : 4;
-    constexpr bool F32 = sizeof(T) == 4;
-    float part[F32 ? NC : 1][4];
+    float part[FRESH ? NC : 1][4];
 #pragma unroll
     for (int x = 0; x < KS; x += Op::KK) {
         typename Op::A a[PARTS];
@@ -143,12 +143,12 @@ __device__ __forceinline__ void add_product(float (&acc)[DP / 8][4], const float
         for (int d = 0; d < NC; d += CB) {
             typename Op::B b[CB];
             Op::load_bk(b, p + x * LD + 8 * d, LD, lane);
-            if constexpr (!F32) Op::template product<false>(acc + d, a, b);
+            if constexpr (!FRESH) Op::template product<false>(acc + d, a, b);
             else if (x == 0) Op::template product<true>(part + d, a, b);
             else Op::template product<false>(part + d, a, b);
         }
     }
-    if constexpr (F32)
+    if constexpr (FRESH)
 #pragma unroll
         for (int d = 0; d < NC; d++)
 #pragma unroll
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(128, ROWS == 16 ? 1 : sizeof(T) == 4 ? 3 : 5) 
                     s[j][2 * r] = x.x, s[j][2 * r + 1] = x.y;
                 }
         }
-        add_product<T, DP, NT * 8, PARTS>(acc, s, BACK ? tk : tv, lane);
+        add_product<T, DP, NT * 8, PARTS, sizeof(T) == 4 || !BACK>(acc, s, BACK ? tk : tv, lane);
     }
     cp_async_wait<0>();
 #pragma unroll
@@ -569,8 +569,8 @@ __global__ void __launch_bounds__(kKeyThreads, sizeof(T) == 4 && DP == 64 ? 2 : 
                     add_at(hq + cb.q * 32, hr + cb.r * 32, hz + cb.z * 32, ds.y);
                 }
             }
-            add_product<T, DP, 32, PARTS>(av, s, tg, lane);
-            add_product<T, DP, 32, PARTS>(ak, dp, tq, lane);
+            add_product<T, DP, 32, PARTS, sizeof(T) == 4>(av, s, tg, lane);
+            add_product<T, DP, 32, PARTS, sizeof(T) == 4>(ak, dp, tq, lane);
         }
     }
     cp_async_wait<0>();
