@@ -140,7 +140,7 @@ class _Problem:
         return s
 
     def buffer(self, nbytes):
-        return torch.empty((nbytes,), dtype=torch.uint8, device=self.q.device) if nbytes else None
+        return self.q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
 
 
 def _ptr(t):
@@ -202,8 +202,10 @@ def _backward(p, dout, saved):
     if saved is not None and saved.numel() != sizes[0]:
         raise ValueError("saved: not of a forward pass of this shape")
     ws = p.buffer(sizes[2])
-    strides = (C.c_int64 * 9)(*gs[:3], *dq.stride()[:3], *dk.stride()[:3])
-    at = C.addressof(strides)
+    row = (3 if nq == n else 2) * h * d  # of packed
+    strides = array("q", (gs[0], gs[1], gs[2], n * row if nq == n else nq * h * d, row if nq == n else h * d, d,
+                          n * row, row, d))
+    at = strides.buffer_info()[0]
     _call(p.dev, "hv_relative_attention_backward", p.arg, dout.data_ptr(), at, _ptr(saved), dq.data_ptr(), dk.data_ptr(),
           dv.data_ptr(), at + 24, at + 48, *(t.data_ptr() for t in tables), _ptr(ws), sizes[2])
     return (dq, dk, dv, *tables), packed
