@@ -165,8 +165,7 @@ __global__ void __launch_bounds__(128, ROWS == 16 ? 1 : sizeof(T) == 4 ? 3 : 5) 
     using Op = Tile<T, DP == 8>;
     constexpr int LD = tile_ld<T, DP>(), NC = DP / 8, THREADS = 128;
     static_assert(ROWS * 2 * WK == THREADS, "a warp for each 16 queries and part of the keys");
-    constexpr int NT = 8 / WK;          // 8-key tiles of a warp
-    constexpr int NB = NT < 4 ? NT : 4;
+    constexpr int NT = 8 / WK;  // 8-key tiles of a warp: 4 or 2
     // The output before rounding gives the backward pass its sum_j p dp, which it
     // takes from every dp: there the probabilities need all 24 bits.
     constexpr int PARTS = BACK || sizeof(T) == 4 ? kParts<T> : __is_same(T, __half) ? 2 : 3;
@@ -266,27 +265,8 @@ __global__ void __launch_bounds__(128, ROWS == 16 ? 1 : sizeof(T) == 4 ? 3 : 5) 
             for (int j = 0; j < NT; j++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) dp[j][e] = -delta[e >> 1];
-#pragma unroll
-        for (int d = 0; d < DP; d += Op::KD) {
-            typename Op::A qa[1];
-            Op::load_a(qa[0], sq + row0 * LD + d, LD, lane);
-#pragma unroll
-            for (int j = 0; j < NT; j += NB) {
-                typename Op::B kb[NB];
-                Op::load_bn(kb, tk + j * 8 * LD + d, LD, lane);
-                if (d == 0) Op::template product_d<true>(s + j, qa, kb);
-                else Op::template product_d<false>(s + j, qa, kb);
-            }
-            if constexpr (BACK) {
-                Op::load_a(qa[0], sg + row0 * LD + d, LD, lane);
-#pragma unroll
-                for (int j = 0; j < NT; j += NB) {
-                    typename Op::B vb[NB];
-                    Op::load_bn(vb, tv + j * 8 * LD + d, LD, lane);
-                    Op::template product_d<false>(dp + j, qa, vb);
-                }
-            }
-        }
+        Op::template dot<true, DP, NT>(s, sq + row0 * LD, tk, LD, lane);
+        if constexpr (BACK) Op::template dot<false, DP, NT>(dp, sg + row0 * LD, tv, LD, lane);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
             const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];
@@ -536,18 +516,8 @@ __global__ void __launch_bounds__(kKeyThreads, sizeof(T) == 4 && DP == 64 ? 2 : 
                 const float4 x = *reinterpret_cast<const float4*>(td + 8 * j + 2 * t);
                 dp[j][0] = dp[j][2] = x.y, dp[j][1] = dp[j][3] = x.w;
             }
-#pragma unroll
-            for (int d = 0; d < DP; d += Op::KD) {
-                typename Op::A ka[1];
-                typename Op::B qb[4];
-                Op::load_a(ka[0], sk + key0 * LD + d, LD, lane);
-                Op::load_bn(qb, tq + d, LD, lane);
-                if (d == 0) Op::template product_d<true>(s, ka, qb);
-                else Op::template product_d<false>(s, ka, qb);
-                Op::load_a(ka[0], sv + key0 * LD + d, LD, lane);
-                Op::load_bn(qb, tg + d, LD, lane);
-                Op::template product_d<false>(dp, ka, qb);
-            }
+            Op::template dot<true, DP, 4>(s, sk + key0 * LD, tq, LD, lane);
+            Op::template dot<false, DP, 4>(dp, sv + key0 * LD, tg, LD, lane);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int4 ma = tm[8 * j + 2 * t], mb = tm[8 * j + 2 * t + 1];

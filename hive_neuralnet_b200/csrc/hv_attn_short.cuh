@@ -228,26 +228,11 @@ __global__ void __launch_bounds__(256) k_attn_short(const AttnArgs a, const Shor
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) s[i][e] = dp[i][e] = 0.f;
-#pragma unroll
-                for (int d = 0; d < DP; d += Op::KD) {
-                    typename Op::A qa[1];
-                    typename Op::B kb[2];
-                    Op::load_a(qa[0], Q + m0 * ld + d, ld, lane);
-                    Op::load_bn(kb, K + d, ld, lane);
-                    Op::template product_d<false>(s, qa, kb);
-                    if (n > 16) {
-                        Op::load_bn(kb, K + 16 * ld + d, ld, lane);
-                        Op::template product_d<false>(s + 2, qa, kb);
-                    }
-                    if (BACK) {
-                        Op::load_a(qa[0], G + m0 * ld + d, ld, lane);
-                        Op::load_bn(kb, V + d, ld, lane);
-                        Op::template product_d<false>(dp, qa, kb);
-                        if (n > 16) {
-                            Op::load_bn(kb, V + 16 * ld + d, ld, lane);
-                            Op::template product_d<false>(dp + 2, qa, kb);
-                        }
-                    }
+                Op::template dot<false, DP, 2>(s, Q + m0 * ld, K, ld, lane);
+                if (n > 16) Op::template dot<false, DP, 2>(s + 2, Q + m0 * ld, K + 16 * ld, ld, lane);
+                if (BACK) {
+                    Op::template dot<false, DP, 2>(dp, G + m0 * ld, V, ld, lane);
+                    if (n > 16) Op::template dot<false, DP, 2>(dp + 2, G + m0 * ld, V + 16 * ld, ld, lane);
                 }
                 int q4[2][3];
 #pragma unroll

@@ -129,6 +129,19 @@ struct Tile {  // 16-bit types
             }
         }
     }
+    // c[i] = (FIRST ? 0 : c[i]) + 16 rows at a times 8 NB rows at b, along DP values
+    template <bool FIRST, int DP, int NB>
+    __device__ static void dot(float (*c)[4], const T* a, const T* b, int ld, int lane) {
+#pragma unroll
+        for (int d = 0; d < DP; d += KD) {
+            A x[1];
+            B y[NB];
+            load_a(x[0], a + d, ld, lane);
+            load_bn(y, b + d, ld, lane);
+            if (d == 0) product_d<FIRST>(c, x, y);
+            else product_d<false>(c, x, y);
+        }
+    }
     // 16 rows x KD values at p (row-major, ld elements a row)
     __device__ static void load_a(A& a, const T* p, int ld, int lane) {
         if constexpr (D8) ldsm2(a.r[0], a.r[1], p + (lane & 15) * ld);
@@ -201,8 +214,38 @@ struct Tile<float, D8> {
 #pragma unroll
         for (int i = 0; i < N; i++) mma_tf32<false>(c[i], a[0].hi, b[i].hi);
     }
-    template <bool FIRST, int N>
-    __device__ static void product_d(float (*c)[4], const A (&a)[1], const B (&b)[N]) { product<FIRST>(c, a, b); }
+    // The tensor core cuts its sums off instead of rounding them: the small
+    // terms are summed by themselves, so that the large sums are cut a third as often.
+    template <bool FIRST, int DP, int NB>
+    __device__ static void dot(float (*c)[4], const float* a, const float* b, int ld, int lane) {
+        float low[NB][4];
+#pragma unroll
+        for (int d = 0; d < DP; d += KD) {
+            A x;
+            B y[NB];
+            load_a(x, a + d, ld, lane);
+            load_bn(y, b + d, ld, lane);
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                if (d == 0) mma_tf32<true>(low[i], x.lo, y[i].hi);
+                else mma_tf32<false>(low[i], x.lo, y[i].hi);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                if (d == 0) mma_tf32<FIRST>(c[i], x.hi, y[i].hi);
+                else mma_tf32<false>(c[i], x.hi, y[i].hi);
+            }
+#pragma unroll
+            for (int i = 0; i < NB; i++) mma_tf32<false>(low[i], x.hi, y[i].lo);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                const float2 z = add2(make_float2(c[i][e], c[i][e + 1]), make_float2(low[i][e], low[i][e + 1]));
+                c[i][e] = z.x, c[i][e + 1] = z.y;
+            }
+    }
     __device__ static void load_a(A& a, const float* p, int ld, int lane) {
         const float* q = p + (lane >> 2) * ld + 2 * (lane & 3);
         const float2 x = *reinterpret_cast<const float2*>(q), y = *reinterpret_cast<const float2*>(q + 8 * ld);
